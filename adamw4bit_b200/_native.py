@@ -21,7 +21,7 @@ F32, BF16, F16 = 0, 1, 2
 RTN, SR_VALUE, SR_UPDATE, FP32_MOMENT = 0, 1, 2, 3
 BLOCK = 128
 LUT_BINS = 1024
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -100,6 +100,20 @@ SIGNATURES = {
     "aw4_unpack_codes": ([_VP, _I64, _VP, _I32, _VP], _I32),
     "aw4_reduce_multicast": ([_VP, _I32, _I64, _F, _VP, _I32, _VP], _I32),
     "aw4_selfcheck_math": ([_VP, _I32, _VP], _I32),
+    "aw4_act8_quantize": ([_VP, _I32, _I64, _I64, _I64, _VP, _VP, _I32, _VP], _I32),
+    "aw4_act8_dequantize": ([_VP, _VP, _I32, _I64, _I64, _VP, _I64, _I32, _VP], _I32),
+    "aw4_swiglu_forward": ([_VP, _VP, _I32, _I64, _I64, _I64, _I64, *[_VP] * 7, _I32, _VP], _I32),
+    "aw4_swiglu_backward": ([_VP, _I32, _I64, _I64, _I64, *[_VP] * 6, _I64, _I32, _VP], _I32),
+    "aw4_rms_norm_forward": ([_VP, _I32, _I64, _I64, _I64, _VP, _I32, _F, *[_VP] * 6, _I32, _VP], _I32),
+    "aw4_rms_norm_backward_workspace": ([_I64, _I64, _I32], _U64),
+    "aw4_rms_norm_backward": ([_VP, _I32, _I64, _I64, _I64, *[_VP] * 4, _I32, _VP, _VP, _VP, _I64, _I32,
+                               _VP], _I32),
+    "aw4_weight_grad_workspace": ([_I64, _I64, _I64, _I64, _I32], _U64),
+    "aw4_weight_grad": ([_VP, _I32, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _VP, _I32, _I32, _VP, _I64,
+                         _VP, _I32, _VP], _I32),
+    "aw4_route_forward_workspace": ([_I64, _I32, _I32], _U64),
+    "aw4_route_forward": ([_VP, _I32, _I64, _I32, _I64, _I32, _VP, _I32, *[_VP] * 6, _I64, _I32, _VP], _I32),
+    "aw4_route_backward": ([_VP, _I32, _I64, _I32, _I64, _I32, _I32, *[_VP] * 7, _I32, _VP], _I32),
 }
 
 

@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define AW4_ABI_VERSION 5
+#define AW4_ABI_VERSION 6
 #define AW4_BLOCK 128          /* elements per quantization block (4-bit default) */
 #define AW4_LUT_BINS 1024      /* maximum uniform bins over [-1, 1] for the rounding search */
 
@@ -209,6 +209,79 @@ int32_t aw4_reduce_multicast(const void* mc, int32_t dtype, int64_t numel, float
  * counts [reciprocal, square root].  No reference counterpart: it validates
  * this build's arithmetic on the running GPU. */
 int32_t aw4_selfcheck_math(uint64_t* counts, int32_t device, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit activation checkpoints (no counterpart in the reference).
+ *
+ * A matrix of rows x cols values is held as codes[rows][pitch], pitch = cols
+ * rounded up to 32 (zeros behind the last column), and scales[rows][pitch/32]:
+ * value = code * 2^(scale - 127), code a signed byte in [-127, 127]; scale 255
+ * marks a block that was not finite and reads back as NaN.  codes 16-byte
+ * aligned.  dtype is that of the values; ld their row stride in values (rows
+ * may start anywhere; 16-byte aligned rows take vector accesses).
+ * ------------------------------------------------------------------------- */
+int32_t aw4_act8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                          uint8_t* codes, uint8_t* scales, int32_t device, void* stream);
+int32_t aw4_act8_dequantize(const uint8_t* codes, const uint8_t* scales, int32_t dtype, int64_t rows,
+                            int64_t cols, void* out, int64_t ld, int32_t device, void* stream);
+
+/* h = gate sigmoid(gate) up (h contiguous) and the checkpoints of gate and up;
+ * hcodes/hscales: NULL, or the checkpoint of h.  Backward reads the two
+ * checkpoints and writes dgate and dup with row stride ld_out. */
+int32_t aw4_swiglu_forward(const void* gate, const void* up, int32_t dtype, int64_t rows, int64_t cols,
+                           int64_t ld_gate, int64_t ld_up, void* h, uint8_t* gcodes, uint8_t* gscales,
+                           uint8_t* ucodes, uint8_t* uscales, uint8_t* hcodes, uint8_t* hscales,
+                           int32_t device, void* stream);
+int32_t aw4_swiglu_backward(const void* dh, int32_t dtype, int64_t rows, int64_t cols, int64_t ld_dh,
+                            const uint8_t* gcodes, const uint8_t* gscales, const uint8_t* ucodes,
+                            const uint8_t* uscales, void* dgate, void* dup, int64_t ld_out,
+                            int32_t device, void* stream);
+
+/* y = x r w, r = rstd[row] = (mean(x^2) + eps)^-1/2, and the checkpoint of x;
+ * cols at most 16384; y contiguous; ycodes/yscales: NULL, or the checkpoint of
+ * y.  Backward: dx = r w dy - v r^3 mean(v w dy) (contiguous), dweight = sum
+ * over rows of dy v r, v the checkpoint's values; workspace of the size that
+ * aw4_rms_norm_backward_workspace gives, contents free. */
+int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                             const void* weight, int32_t weight_dtype, float eps, void* y, float* rstd,
+                             uint8_t* codes, uint8_t* scales, uint8_t* ycodes, uint8_t* yscales,
+                             int32_t device, void* stream);
+uint64_t aw4_rms_norm_backward_workspace(int64_t rows, int64_t cols, int32_t device);
+int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                              const uint8_t* codes, const uint8_t* scales, const float* rstd,
+                              const void* weight, int32_t weight_dtype, void* dx, void* dweight,
+                              float* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+
+/* out[g][n][k] (+)= sum over rows t in [offsets[g], offsets[g + 1]) of
+ * dy[t][n] v[t][k], v the checkpoint's values; offsets: NULL for one group of
+ * all rows, else groups + 1 device integers (cut to [0, rows]).  dtype bf16 or
+ * f16; out_dtype the same or f32. */
+uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device);
+int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
+                        const uint8_t* codes, const uint8_t* scales, int64_t k, const int32_t* offsets,
+                        int64_t groups, void* out, int32_t out_dtype, int32_t accumulate,
+                        void* workspace, int64_t workspace_bytes, int32_t* status, int32_t device,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Expert router (no counterpart in the reference): softmax over the experts,
+ * the k largest logits (ties to the lowest index; -inf never), their weights,
+ * counts[experts] with the number of valid rows behind them (experts + 1
+ * integers) and the balance loss sum_e (E counts_e / (k n)) mean(p_e).
+ * valid: NULL or one byte a row.  stats: two floats a row for the backward
+ * call, 8-byte aligned.  Rows that are not valid, or all -inf: choices -1,
+ * weights and gradients 0.  dweights and dbalance: NULL for zero.
+ * ------------------------------------------------------------------------- */
+#define AW4_ROUTE_MAX_EXPERTS 1024
+uint64_t aw4_route_forward_workspace(int64_t rows, int32_t experts, int32_t device);
+int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
+                          int32_t k, const uint8_t* valid, int32_t renormalize, float* weights,
+                          int32_t* chosen, float* stats, int32_t* counts, float* balance,
+                          void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
+                           int32_t k, int32_t renormalize, const float* weights, const int32_t* chosen,
+                           const float* stats, const int32_t* counts, const float* dweights,
+                           const float* dbalance, void* dlogits, int32_t device, void* stream);
 
 #ifdef __cplusplus
 }
