@@ -147,6 +147,20 @@ def check(rc: int, what: str) -> None:
         raise NativeError(f"{what}: {kind}: {msg}")
 
 
+_wait_status: torch.Tensor | None = None
+
+
+def wait_status() -> int:
+    """Address of the pinned word that a kernel sets when one of its waits runs out.  It is looked at before
+    each launch that passes it: the outputs of the launch that set it are not to be used."""
+    global _wait_status
+    if _wait_status is None:
+        _wait_status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    elif ctypes.c_int32.from_address(_wait_status.data_ptr()).value:
+        raise NativeError("a kernel of an earlier call gave up a wait; its outputs are not complete")
+    return _wait_status.data_ptr()
+
+
 def launch_count() -> int:
     return int(lib().aw4_launch_count())
 

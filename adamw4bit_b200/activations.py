@@ -405,11 +405,16 @@ def weight_grad(dy: torch.Tensor, x8: Act8, offsets: torch.Tensor | None = None,
             raise ValueError(f"weight_grad: contiguous out of shape {shape} expected, found {tuple(out.shape)}")
     if out.dtype not in (dy.dtype, torch.float32):
         raise TypeError(f"weight_grad: result in {dy.dtype} or float32 expected, found {out.dtype}")
+    if rows and (ld < n or ld % 8 or src.data_ptr() % 16):
+        # the bulk copies want rows on 16 bytes
+        padded = torch.empty((rows, -(-n // 8) * 8), dtype=dy.dtype, device=dev)
+        padded[:, :n].copy_(src.reshape(rows, n))
+        src, ld = padded, padded.shape[1]
     nbytes = _wgrad_workspace(rows, n, k, groups, dev.index)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     N.check(N.lib().aw4_weight_grad(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, n, ld, *x8._ptrs(), k,
                                     N.ptr(offsets), groups, out.data_ptr(), N.DTYPE_CODES[out.dtype],
-                                    int(accumulate), N.ptr(ws), nbytes, None, dev.index, N.stream_handle(dev)),
+                                    int(accumulate), N.ptr(ws), nbytes, N.wait_status(), dev.index, N.stream_handle(dev)),
             "aw4_weight_grad")
     return out
 
