@@ -19,6 +19,23 @@ __device__ __forceinline__ void bar_init(uint32_t bar, int arrivals) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The barrier at the same place in the pair's first block.
+__device__ __forceinline__ uint32_t in_first_block(uint32_t bar) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ uint32_t block_in_pair() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -76,15 +93,20 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
-// ---- tensor memory and tensor core -------------------------------------------
+// ---- tensor memory and tensor core, in pairs of blocks ------------------------
+//
+// A pair's product is 256 x n: each block holds 128 of the rows in its tensor
+// memory, those rows of the first operand and half the columns of the second in its shared
+// memory.  One thread of the pair's first block issues for both.
 
+// Both by the same warp of each block of the pair.
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, int cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(cols)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(cols)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_free(uint32_t taddr, int cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -92,14 +114,16 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// The barrier gets one arrival when every tcgen05.mma issued so far by this thread is done.
+// The barrier of both blocks gets one arrival when every product issued so far by this thread is done.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
         "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n"
-        "  tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+        "  tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
 // 32 columns of this warp's 32 lanes.
@@ -126,11 +150,11 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t column_strid
 }
 
 // Instruction descriptor: float32 sums, both operands with their columns
-// contiguous (the inner dimension strided), 128 x n.
+// contiguous (the inner dimension strided), 256 x n.
 __device__ __forceinline__ uint32_t tc_idesc(bool bf16, int n) {
     const uint32_t type = bf16 ? 1u : 0u;
     return (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(n >> 3) << 17) |
-           ((128u >> 4) << 24);
+           ((256u >> 4) << 24);
 }
 
 }  // namespace aw4

@@ -4,15 +4,21 @@
 // checkpoint's values.  Group g holds rows [offsets[g], offsets[g + 1]); an
 // empty group's gradient is zero.
 //
-// A block holds a 256 x 256 tile of dW in tensor memory (two 128 x 256
-// accumulators, all 512 columns) and walks the rows 64 at a time:
+// A pair of blocks holds a 512 x 256 tile of dW in tensor memory (two 256 x 256
+// accumulators, 128 rows of each in a block: all 512 columns) and walks the rows 64
+// at a time.  In each block:
 //
-//   warp 8      bulk tensor copies of dy [64][256] and of the codes [64][256] bytes, three stages
-//   warps 0-7   codes * 2^e -> 16-bit values in shared memory, two buffers.  A lane owns
-//               64 values of one row, a 128-byte line of the operand: reads and
-//               writes of a warp then cover all banks under the 128-byte swizzle
-//   warp 9      tcgen05.mma, both operands with the row index as the inner dimension
-//   warps 0-7   accumulators -> dW, or a float32 partial tile
+//   warp 16      bulk tensor copies of its dy [64][256] and codes [64][128], four stages
+//   warps 0-15   codes * 2^e -> 16-bit values in shared memory, three buffers, two groups
+//                of warps taking turns.  A lane owns a block of 32 codes of one row
+//   warp 17      (first block) tcgen05.mma for the pair, both operands with the row
+//                index as the inner dimension
+//   warps 0-15   accumulators -> dW, or a float32 partial tile
+//
+// A pair, because shared memory bounds a single block: for 256 x 256 x 64 its tensor
+// core reads 96 KB of operands, and copies and conversion move 96 KB more, 1536
+// cycles at 128 bytes a cycle for 1024 cycles of products.  A pair's tensor cores share
+// the values, so that a block moves 128 KB in the same 1024 cycles.
 //
 // q * 2^e is exact in bf16 and f16, so the products are those of dy and the
 // checkpoint's own values, summed in float32.
@@ -20,9 +26,9 @@
 // Rows behind a group's last are zeroed in both operands (a NaN of the next
 // group must not meet a zero).
 //
-// Work split: whole tiles go round the blocks, n-tiles outermost so that
-// blocks that run together share dy and codes in L2; the last wave and what
-// does not fill one are cut by row steps, so that every block gets the same
+// Work split: whole tiles go round the pairs, n-tiles outermost so that
+// pairs that run together share dy and codes in L2; the last wave and what
+// does not fill one are cut by row steps, so that every pair gets the same
 // number of steps whatever the groups' sizes.  A tile that is cut leaves float32
 // partial tiles, added in the order of their rows by a second kernel: the same bits
 // on every run.
@@ -39,16 +45,18 @@
 
 namespace aw4 {
 
-constexpr int kWgTile = 256;                 // n and k of a tile
-constexpr int kWgRows = 64;                  // rows of a step
-constexpr int kWgStages = 3;
-constexpr int kWgConvert = 256;              // threads that convert and write out
+constexpr int kWgTileN = 512, kWgTileK = 256;   // a pair's tile
+constexpr int kWgRows = 64;                     // rows of a step
+constexpr int kWgStages = 4, kWgBuffers = 3;
+constexpr int kWgConvert = 512;                 // threads that convert and write out, in two groups
 constexpr int kWgThreads = kWgConvert + 64;
-constexpr int kWgDyBytes = kWgRows * kWgTile * 2;
-constexpr int kWgCodeBytes = kWgRows * kWgTile;
-constexpr int kWgBox = kWgRows * 128;        // a copied box: 64 lines of 128 bytes
-constexpr int kWgMaxBlocks = 256;            // the schedule's scan gives a thread to each block
-constexpr int kWgSegments = 2 * kWgMaxBlocks + 2;
+constexpr int kWgCopy = kWgConvert / 32, kWgProduct = kWgCopy + 1;   // warps
+constexpr int kWgBox = kWgRows * 128;           // a copied box: 64 lines of 128 bytes
+constexpr int kWgDyBytes = 4 * kWgBox;          // a block's 2 x 128 columns of dy
+constexpr int kWgCodeBytes = kWgBox;            // its 128 codes of each row
+constexpr int kWgValBytes = 2 * kWgBox;         // ... and their values
+constexpr int kWgMaxPairs = 128;
+constexpr int kWgMaxCut = 2 * kWgMaxPairs;      // cut tiles: less than two for each pair
 
 struct WgSegment {
     int tile;         // over all groups
@@ -78,16 +86,21 @@ struct WgParams {
 };
 
 struct WgShared {
-    alignas(8) uint64_t full[kWgStages], empty[kWgStages], ready[2], done[2], acc_full, acc_empty, drain;
+    alignas(8) uint64_t full[kWgStages], empty[kWgStages], ready[kWgBuffers], done[kWgBuffers], acc_full, acc_empty,
+        out_done, drain;
     uint32_t tmem;
     int gave_up;
-    int segments;
-    int whole;                  // whole tiles of this block
-    int64_t scan[kWgMaxBlocks];
-    WgSegment list[kWgSegments];
+    int whole;                  // whole tiles of this pair
+    int first_cut, cuts;        // its segments of cut tiles: entries of `list`
+    int64_t part[3][kWgThreads / 32];
+    WgSegment list[kWgMaxCut];
 };
 
-constexpr int kWgSmem = 1024 + kWgStages * (kWgDyBytes + kWgCodeBytes) + 2 * kWgDyBytes + (int)sizeof(WgShared);
+constexpr int kWgSmem =
+    1024 + kWgStages * (kWgDyBytes + kWgCodeBytes) + kWgBuffers * kWgValBytes + (int)sizeof(WgShared);
+static_assert(kWgSmem <= 227 * 1024, "shared memory of a block");
+static_assert(kWgConvert / 32 * 2048 <= kWgBuffers * kWgValBytes, "2 KB for each warp that writes out");
+static_assert(kWgMaxCut <= kWgThreads, "a thread for each cut tile");
 
 __device__ __forceinline__ void wg_group(const WgParams& p, int g, int64_t& first, int64_t& last) {
     first = 0;
@@ -105,85 +118,80 @@ __device__ __forceinline__ int wg_steps(const WgParams& p, int g) {
     return max(1, (int)((last - first + kWgRows - 1) / kWgRows));
 }
 
-// This block's segments of the cut tiles.  Tiles [cut, tiles) are laid end to end as
-// row steps; block b takes as many as it lacks to the average of all blocks.
-__device__ void wg_schedule(const WgParams& p, WgShared& s) {
-    const int tid = threadIdx.x;
+// Sum over the block, for every thread; `slot` names scratch of its own.
+__device__ __forceinline__ int64_t wg_block_sum(int64_t v, int64_t* part) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < kWgThreads / 32; ++i) v += part[i];
+    __syncthreads();
+    return v;
+}
+
+// This pair's segments.  Tiles [cut, tiles) are laid end to end as row steps; a pair
+// takes as many as it lacks to the average of all pairs.  A thread looks at one pair, then at one cut tile.
+__device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs, bool writes) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_group = p.n_tiles * p.k_tiles;
     const int tiles = per_group * p.groups;
-    const int blocks = gridDim.x;
-    const int whole = max(0, tiles / blocks - 1);      // whole tiles of every block
-    const int cut = whole * blocks;
-    int64_t mine = 0;
-    if (tid < blocks) {
-        if (p.offsets)
-            for (int w = 0; w < whole; ++w) mine += wg_steps(p, (w * blocks + tid) / per_group);
-        else
-            mine = (int64_t)whole * wg_steps(p, 0);
+    const int whole = max(0, tiles / pairs - 1);       // whole tiles of every pair
+    const int cut = whole * pairs;
+    int64_t load = 0;
+    if (tid < pairs) {
+        if (p.offsets) {
+#pragma unroll 8
+            for (int w = 0; w < whole; ++w) load += wg_steps(p, (w * pairs + tid) / per_group);
+        } else {
+            load = (int64_t)whole * wg_steps(p, 0);
+        }
     }
-    if (tid < kWgMaxBlocks) s.scan[tid] = mine;
+    const int steps = cut + tid < tiles ? wg_steps(p, (cut + tid) / per_group) : 0;
+    if (tid == 0) s.first_cut = kWgMaxCut;
+    if (tid == 1) s.cuts = 0;
+    const int64_t rest = wg_block_sum(steps, s.part[0]);
+    const int64_t target = (wg_block_sum(load, s.part[1]) + rest + pairs - 1) / pairs;
+    const int64_t lack = tid < pairs ? max((int64_t)0, target - load) : 0;
+    const int64_t from = min(rest, wg_block_sum(tid < pair ? lack : 0, s.part[0]));
+    const int64_t to = min(rest, from + wg_block_sum(tid == pair ? lack : 0, s.part[1]));
+    // where this thread's tile begins
+    int64_t at = steps;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+    }
+    if (lane == 31) s.part[2][warp] = at;
     __syncthreads();
-    if (tid == 0) {
-        int64_t load = 0, rest = 0;
-        for (int b = 0; b < blocks; ++b) load += s.scan[b];
-        for (int t = cut; t < tiles;) {
-            const int g = t / per_group, end = min(tiles, (g + 1) * per_group);
-            rest += (int64_t)(end - t) * wg_steps(p, g);
-            t = end;
-        }
-        const int64_t target = (load + rest + blocks - 1) / blocks;
-        int64_t from = 0;
-        for (int b = 0; b < (int)blockIdx.x; ++b) from += max((int64_t)0, target - s.scan[b]);
-        int64_t to = from + max((int64_t)0, target - s.scan[blockIdx.x]);
-        from = min(from, rest);
-        to = min(to, rest);
-        int count = 0;
-        WgSlot first_slot = {-1, 0}, last_slot = {-1, 0};
-        int64_t at = 0;
-        for (int t = cut; from < to && t < tiles && at < to;) {
-            const int g = t / per_group, end = min(tiles, (g + 1) * per_group);
-            const int steps = wg_steps(p, g);
-            const int64_t group_end = at + (int64_t)(end - t) * steps;
-            if (group_end > from) {
-                if (from > at) {
-                    const int skip = (int)((from - at) / steps);
-                    t += skip;
-                    at += (int64_t)skip * steps;
-                }
-                for (; t < end && at < to && count < kWgSegments; ++t, at += steps) {
-                    const int a = (int)max((int64_t)0, from - at), b = (int)min((int64_t)steps, to - at);
-                    int slot = -1;
-                    if (a > 0) {
-                        slot = 2 * blockIdx.x;
-                        first_slot = {t, b == steps};
-                    } else if (b < steps) {
-                        slot = 2 * blockIdx.x + 1;
-                        last_slot = {t, 0};
-                    }
-                    s.list[count++] = {t, a, b, slot};
-                }
-            }
-            at = group_end;
-            t = end;
-        }
-        s.segments = count;
-        s.whole = whole;
-        p.slots[2 * blockIdx.x] = first_slot;
-        p.slots[2 * blockIdx.x + 1] = last_slot;
+    at -= steps;
+    for (int i = 0; i < warp; ++i) at += s.part[2][i];
+    if (writes && tid < 2) p.slots[2 * pair + tid] = {-1, 0};
+    __syncthreads();
+    const int64_t a = max(from, at), b = min(to, at + steps);
+    if (a < b) {
+        const int first = (int)(a - at), last = (int)(b - at);
+        const int slot = first > 0 ? 2 * pair : last < steps ? 2 * pair + 1 : -1;
+        s.list[tid] = {cut + tid, first, last, slot};
+        atomicMin(&s.first_cut, tid);
+        atomicAdd(&s.cuts, 1);
+        if (writes && slot >= 0) p.slots[slot] = {cut + tid, last == steps};
     }
+    if (tid == 0) s.whole = whole;
     __syncthreads();
 }
 
-__device__ __forceinline__ WgSegment wg_segment(const WgParams& p, const WgShared& s, int i) {
-    if (i >= s.whole) return s.list[i - s.whole];
-    const int tile = i * gridDim.x + blockIdx.x;
+__device__ __forceinline__ WgSegment wg_segment(const WgParams& p, const WgShared& s, int i, int pair, int pairs) {
+    if (i >= s.whole) return s.list[s.first_cut + i - s.whole];
+    const int tile = i * pairs + pair;
     return {tile, 0, wg_steps(p, tile / (p.n_tiles * p.k_tiles)), -1};
 }
 
 struct WgTile {
     int g, n0, k0;
     int64_t first, last;
-    int dy_boxes, code_boxes;   // boxes of 64 columns of dy, of 128 of the codes
+    int half;         // columns of k that a block converts: the product has twice as many
 };
 
 __device__ __forceinline__ WgTile wg_tile(const WgParams& p, int tile) {
@@ -191,11 +199,10 @@ __device__ __forceinline__ WgTile wg_tile(const WgParams& p, int tile) {
     const int per_group = p.n_tiles * p.k_tiles;
     t.g = tile / per_group;
     const int in = tile - t.g * per_group;
-    t.n0 = in / p.k_tiles * kWgTile;
-    t.k0 = in % p.k_tiles * kWgTile;
+    t.n0 = in / p.k_tiles * kWgTileN;
+    t.k0 = in % p.k_tiles * kWgTileK;
     wg_group(p, t.g, t.first, t.last);
-    t.dy_boxes = min(4, (p.n - t.n0 + 63) / 64);
-    t.code_boxes = min(2, (p.k - t.k0 + 127) / 128);
+    t.half = p.k - t.k0 > 128 ? 128 : 64;
     return t;
 }
 
@@ -209,58 +216,91 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// 64 codes of row r, columns [64 c, 64 c + 64) of the step, to 16-bit values.
+// Block j of 32 codes of row r of the step, to 16-bit values.  A quarter of a
+// warp has two rows and four blocks: the order of a block's halves, and the
+// swizzle, put its eight accesses on different banks.
 template <int DT>
-__device__ __forceinline__ void wg_convert(const char* codes, char* operand, int r, int c, int b0, int b1,
-                                           bool live) {
-    char* line = operand + c * kWgBox + r * 128;
-    const int swz = r & 7;
-    if (!live) {
+__device__ __forceinline__ void wg_convert(const char* codes, char* operand, int r, int j, int byte, bool live) {
+    char* line = operand + (j >> 1) * kWgBox + r * 128;
+    const int swz = r & 7, to = (j & 1) * 4;
+    const float s = a8_scale(byte);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + j * 16) = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    const char* src = codes + (c >> 1) * kWgBox + r * 128;
-    const float s[2] = {a8_scale(b0), a8_scale(b1)};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + ((((c & 1) * 4 + j) ^ swz) << 4));
+    for (int i = 0; i < 2; ++i) {
+        const int h = i ^ (j >> 1);
+        uint4 w = *reinterpret_cast<const uint4*>(codes + r * 128 + (((2 * j + h) ^ swz) << 4));
         const uint32_t q[4] = {w.x, w.y, w.z, w.w};
         uint32_t o[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int k = 0; k < 4; ++k) {
             float v[4];
-            a8_decode4(q[i], s[j >> 1], v);
-            o[2 * i] = pack2<DT>(v[0], v[1]);
-            o[2 * i + 1] = pack2<DT>(v[2], v[3]);
+            a8_decode4(q[k], s, v);
+            o[2 * k] = live ? pack2<DT>(v[0], v[1]) : 0u;
+            o[2 * k + 1] = live ? pack2<DT>(v[2], v[3]) : 0u;
         }
-        *reinterpret_cast<uint4*>(line + (((2 * j) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(line + (((2 * j + 1) ^ swz) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        *reinterpret_cast<uint4*>(line + (((to + 2 * h) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(line + (((to + 2 * h + 1) ^ swz) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
     }
 }
 
-// 32 sums of one row of dW.
-template <int OT>
-__device__ __forceinline__ void wg_store(const WgParams& p, int64_t row_off, int k, const uint32_t v[32]) {
+// Stores 16 bytes' worth of a row of dW: 4 float32 sums (FROM32), rounded and, with `accumulate`, added to
+// what is there, or 8 values that are rounded already.
+template <int OT, bool FROM32>
+__device__ __forceinline__ void wg_store(const WgParams& p, int64_t row_off, int k, uint4 w) {
+    constexpr int kCount = FROM32 ? 4 : 8;
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const bool whole = p.vec_out && k + kCount <= p.k;
+    if constexpr (!FROM32) {
+        uint16_t* o = static_cast<uint16_t*>(p.out) + row_off + k;
+        if (whole) {
+            __stcs(reinterpret_cast<uint4*>(o), w);
+        } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int at = k + c * 8;
-        if (at >= p.k) return;
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[c * 8 + i]);
-        if (p.accumulate) {
-            float o[8];
-            widen8<OT>(load_raw8<OT>(p.out, row_off, at, p.k, p.vec_out), o);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += o[i];
+            for (int i = 0; i < 8; ++i)
+                if (k + i < p.k) o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
         }
-        store_raw8<OT>(p.out, row_off, at, p.k, p.vec_out, narrow8<OT>(f));
+    } else if (OT == AW4_F32 && whole && !p.accumulate) {
+        __stcs(reinterpret_cast<uint4*>(static_cast<uint32_t*>(p.out) + row_off + k), w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k + i < p.k) {
+                const float f = __uint_as_float(v[i]);
+                const int64_t at = row_off + k + i;
+                Elem<OT>::store1(p.out, at, p.accumulate ? Elem<OT>::load1(p.out, at) + f : f);
+            }
     }
+}
+
+// 32 lines of 64 bytes, a line a lane, turned in the warp's shared memory so
+// that four lanes store a line: whole sectors.  Line r is row row0 + r of group g's
+// dW, from column k on.
+template <int OT, bool FROM32>
+__device__ __forceinline__ void wg_store_lines(const WgParams& p, char* stage, int64_t first_row, int rows, int k,
+                                               const uint32_t v[16]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), c = lane & 3;
+        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+        const int at = k + c * (FROM32 ? 4 : 8);
+        if (r < rows && at < p.k) wg_store<OT, FROM32>(p, (first_row + r) * p.k, at, w);
+    }
+}
+
+// A partial tile keeps four columns of all its rows together, so that a warp, a row a lane, writes and
+// reads whole lines.  Four sums at row `row` and column `col` of the tile:
+__device__ __forceinline__ float4* wg_partial(const WgParams& p, int slot, int row, int col) {
+    return reinterpret_cast<float4*>(p.partial) + ((int64_t)slot * (kWgTileK / 4) + col / 4) * kWgTileN + row;
 }
 
 template <int DT, int OT>
-__global__ void __launch_bounds__(kWgThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
 weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map,
                    const WgParams p) {
     extern __shared__ char raw_smem[];
@@ -268,43 +308,57 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
     char* dy_s = base;
     char* code_s = dy_s + kWgStages * kWgDyBytes;
     char* val_s = code_s + kWgStages * kWgCodeBytes;
-    WgShared& s = *reinterpret_cast<WgShared*>(val_s + 2 * kWgDyBytes);
+    WgShared& s = *reinterpret_cast<WgShared*>(val_s + kWgBuffers * kWgValBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int side = block_in_pair();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kWgStages; ++i) {
             bar_init(smem_addr(&s.full[i]), 1);
             bar_init(smem_addr(&s.empty[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            bar_init(smem_addr(&s.ready[i]), kWgConvert / 32);
+        for (int i = 0; i < kWgBuffers; ++i) {
+            bar_init(smem_addr(&s.ready[i]), kWgConvert / 32);   // one group of each block
             bar_init(smem_addr(&s.done[i]), 1);
         }
         bar_init(smem_addr(&s.acc_full), 1);
-        bar_init(smem_addr(&s.acc_empty), kWgConvert / 32);
+        bar_init(smem_addr(&s.acc_empty), 2 * kWgConvert / 32);
+        bar_init(smem_addr(&s.out_done), kWgConvert / 32);
         bar_init(smem_addr(&s.drain), 1);
         s.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) tmem_alloc(smem_addr(&s.tmem), 512);
-    wg_schedule(p, s);
+    if (warp == kWgProduct) tmem_alloc(smem_addr(&s.tmem), 512);
+    wg_schedule(p, s, pair, pairs, side == 0);
     tc_fence_before();
-    __syncthreads();
+    pair_sync();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    const int segments = s.whole + s.segments;
+    const int segments = s.whole + s.cuts;
     volatile int* gave_up = &s.gave_up;
 
-    if (warp == 8) {
+    if (warp == kWgCopy) {
         if (lane == 0) {
             tma_prefetch_map(&dy_map);
             tma_prefetch_map(&code_map);
             uint32_t c = 0;
             bool ok = true;
             for (int i = 0; ok && i < segments; ++i) {
-                const WgSegment seg = wg_segment(p, s, i);
+                const WgSegment seg = wg_segment(p, s, i, pair, pairs);
                 const WgTile t = wg_tile(p, seg.tile);
-                const uint32_t bytes = (t.dy_boxes + t.code_boxes) * kWgBox;
+                const int n1 = t.n0 + side * 128, k1 = t.k0 + side * t.half;
+                // boxes that begin inside the matrices; what lies behind reads as zero or
+                // is multiplied into sums that nobody stores
+                bool in[4];
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    in[b] = n1 + (b >> 1) * 256 + (b & 1) * 64 < p.n;
+                    bytes += in[b] ? kWgBox : 0;
+                }
+                const bool codes_in = k1 < (int)(p.blocks * kA8Block);
+                bytes += codes_in ? kWgBox : 0;
                 for (int step = seg.first; step < seg.last; ++step, ++c) {
                     const int st = c % kWgStages;
                     ok = bar_wait(smem_addr(&s.empty[st]), ((c / kWgStages) & 1) ^ 1, gave_up);
@@ -312,11 +366,12 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                     const uint32_t bar = smem_addr(&s.full[st]);
                     const int row = (int)(t.first + (int64_t)step * kWgRows);
                     bar_expect(bar, bytes);
-                    for (int b = 0; b < t.dy_boxes; ++b)
-                        tma_load_2d(smem_addr(dy_s + st * kWgDyBytes + b * kWgBox), &dy_map, t.n0 + b * 64, row, bar);
-                    for (int b = 0; b < t.code_boxes; ++b)
-                        tma_load_2d(smem_addr(code_s + st * kWgCodeBytes + b * kWgBox), &code_map, t.k0 + b * 128,
-                                    row, bar);
+                    if (codes_in) tma_load_2d(smem_addr(code_s + st * kWgCodeBytes), &code_map, k1, row, bar);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (in[b])
+                            tma_load_2d(smem_addr(dy_s + st * kWgDyBytes + b * kWgBox), &dy_map,
+                                        n1 + (b >> 1) * 256 + (b & 1) * 64, row, bar);
                 }
             }
             if (!ok)   // copies in flight land before the block leaves
@@ -324,24 +379,24 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                     bar_drain(smem_addr(&s.full[j % kWgStages]), (j / kWgStages) & 1);
         }
         __syncwarp();
-    } else if (warp == 9) {
-        if (lane == 0) {
-            uint32_t c = 0;
+    } else if (warp == kWgProduct) {
+        if (lane == 0 && side == 0) {
+            uint32_t c = 0, buf = 0, turn = 0;
             bool ok = true;
             for (int i = 0; ok && i < segments; ++i) {
-                const WgSegment seg = wg_segment(p, s, i);
+                const WgSegment seg = wg_segment(p, s, i, pair, pairs);
                 const WgTile t = wg_tile(p, seg.tile);
-                const uint32_t idesc = tc_idesc(DT == AW4_BF16, min(kWgTile, (p.k - t.k0 + 15) / 16 * 16));
-                const bool two = t.dy_boxes > 2;
+                const uint32_t idesc = tc_idesc(DT == AW4_BF16, 2 * t.half);
+                const bool two = t.n0 + 256 < p.n;
                 ok = bar_wait(smem_addr(&s.acc_empty), (i & 1) ^ 1, gave_up);
                 for (int step = seg.first; ok && step < seg.last; ++step, ++c) {
-                    const int st = c % kWgStages, b = c & 1;
-                    ok = bar_wait(smem_addr(&s.ready[b]), (c >> 1) & 1, gave_up) &&
-                         bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up);
+                    const int st = c % kWgStages;
+                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
+                         bar_wait(smem_addr(&s.ready[buf]), turn, gave_up);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t dy_a = smem_addr(dy_s + st * kWgDyBytes);
-                    const uint32_t val_a = smem_addr(val_s + b * kWgDyBytes);
+                    const uint32_t val_a = smem_addr(val_s + buf * kWgValBytes);
 #pragma unroll
                     for (int j = 0; j < kWgRows / 16; ++j) {
                         const uint64_t vd = tc_desc(val_a + j * 2048, kWgBox);
@@ -350,7 +405,11 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                         if (two) tc_mma_f16(tmem + 256, tc_desc(dy_a + 2 * kWgBox + j * 2048, kWgBox), vd, idesc, add);
                     }
                     tc_commit(smem_addr(&s.empty[st]));
-                    tc_commit(smem_addr(&s.done[b]));
+                    tc_commit(smem_addr(&s.done[buf]));
+                    if (++buf == kWgBuffers) {
+                        buf = 0;
+                        turn ^= 1;
+                    }
                 }
                 if (ok) tc_commit(smem_addr(&s.acc_full));
             }
@@ -361,128 +420,156 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
         }
         __syncwarp();
     } else {
-        const int r = threadIdx.x & 63, chunk = threadIdx.x >> 6;
-        uint32_t c = 0;
+        const int group = warp >> 3;                   // converts the steps of its parity
+        const int r = (warp & 7) * 8 + (lane >> 2), j = lane & 3;
+        uint32_t c = 0, buf = 0, turn = 0;
         bool ok = true;
         for (int i = 0; ok && i < segments; ++i) {
-            const WgSegment seg = wg_segment(p, s, i);
+            const WgSegment seg = wg_segment(p, s, i, pair, pairs);
             const WgTile t = wg_tile(p, seg.tile);
-            const uint32_t block = t.k0 / kA8Block + chunk * 2;
-            const bool cols = chunk < t.code_boxes * 2 && block < p.blocks;
-            const bool second = block + 1 < p.blocks;
-            const int64_t row0 = t.first + (int64_t)seg.first * kWgRows + r;
-            // exponent bytes of the next step are on their way while this one is converted
-            int b0 = 1, b1 = 1;
-            if (cols && row0 < t.last) {
-                b0 = p.scales[row0 * p.blocks + block];
-                if (second) b1 = p.scales[row0 * p.blocks + block + 1];
-            }
+            const uint32_t block = (t.k0 + side * t.half) / kA8Block + j;
+            const bool cols = j * kA8Block < t.half && block < p.blocks;
+            // the exponent of this group's next step is on its way while one is converted
+            const int skip = (c & 1) ^ group;
+            int64_t row = t.first + (int64_t)(seg.first + skip) * kWgRows + r;
+            const int64_t end = min(t.last, t.first + (int64_t)seg.last * kWgRows);
+            const uint8_t* scale = p.scales + row * p.blocks + block;
+            int byte = cols && row < end ? *scale : 1;
+            // the values' buffers also turn the last tile's sums on their way out
+            if (i > 0) ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.out_done), (i - 1) & 1, gave_up));
+            if (!ok) break;
             for (int step = seg.first; step < seg.last; ++step, ++c) {
-                const int st = c % kWgStages, b = c & 1;
-                const int64_t row = t.first + (int64_t)step * kWgRows + r;
-                const bool live = row < t.last;
-                int nb0 = 1, nb1 = 1;
-                if (cols && step + 1 < seg.last && row + kWgRows < t.last) {
-                    nb0 = p.scales[(row + kWgRows) * p.blocks + block];
-                    if (second) nb1 = p.scales[(row + kWgRows) * p.blocks + block + 1];
-                }
-                ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
-                     bar_wait(smem_addr(&s.done[b]), ((c >> 1) & 1) ^ 1, gave_up);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (cols) wg_convert<DT>(code_s + st * kWgCodeBytes, val_s + b * kWgDyBytes, r, chunk, b0, b1, live);
-                if (!live) {   // the row belongs to the next group
-                    char* line = dy_s + st * kWgDyBytes + chunk * kWgBox + r * 128;
+                if ((c & 1) == group) {
+                    const int st = c % kWgStages;
+                    const bool live = row < t.last;
+                    row += 2 * kWgRows;
+                    scale += 2 * kWgRows * p.blocks;
+                    const int next = cols && row < end ? *scale : 1;
+                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
+                         bar_wait(smem_addr(&s.done[buf]), turn ^ 1, gave_up);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (cols) wg_convert<DT>(code_s + st * kWgCodeBytes, val_s + buf * kWgValBytes, r, j, byte, live);
+                    if (!live) {   // the row belongs to the next group
+                        char* line = dy_s + st * kWgDyBytes + j * kWgBox + r * 128;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + j * 16) = make_uint4(0, 0, 0, 0);
+                        for (int h = 0; h < 8; ++h)
+                            *reinterpret_cast<uint4*>(line + h * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    byte = next;
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(in_first_block(smem_addr(&s.ready[buf])));
                 }
-                b0 = nb0;
-                b1 = nb1;
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) bar_arrive(smem_addr(&s.ready[b]));
+                if (++buf == kWgBuffers) {
+                    buf = 0;
+                    turn ^= 1;
+                }
             }
             if (!ok) break;
             ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.acc_full), i & 1, gave_up));
             if (!ok) break;
             tc_fence_after();
-            // warps 0-3: rows 0-127 of the tile, warps 4-7: rows 128-255
-            const int row_in = (warp >> 2) * 128 + (warp & 3) * 32 + lane;
+            // four warps for the 128 rows that this block has of each accumulator; the groups
+            // take half the columns each
+            const int acc = (warp >> 2) & 1;
+            const int row_in = acc * 256 + side * 128 + (warp & 3) * 32 + lane;
             const int n = t.n0 + row_in;
-            const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * 256;
-            const int k_end = min(kWgTile, p.k - t.k0);
-            if (t.n0 + (warp >> 2) * 128 < p.n)
-                for (int col = 0; col < k_end; col += 32) {
+            const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + acc * 256;
+            const int k_end = min(group * 128 + 128, p.k - t.k0);
+            const int64_t first_row = (int64_t)t.g * p.n + n - lane;
+            // no product reads the values any more, and none are written before out_done
+            char* stage = val_s + warp * 2048;
+            if (n - lane < p.n)
+                for (int col = group * 128; col < k_end; col += 32) {
                     uint32_t v[32];
                     tmem_load32(from + col, v);
                     tmem_load_wait();
-                    if (n < p.n) {
-                        if (seg.slot < 0) {
-                            wg_store<OT>(p, ((int64_t)t.g * p.n + n) * p.k, t.k0 + col, v);
-                        } else {
-                            float4* o = reinterpret_cast<float4*>(
-                                p.partial + ((int64_t)seg.slot * kWgTile + row_in) * kWgTile + col);
+                    if (seg.slot >= 0) {
+                        float4* o = wg_partial(p, seg.slot, row_in, col);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                o[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                                   __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-                        }
+                        for (int q = 0; q < 8; ++q)
+                            if (n < p.n)
+                                o[q * kWgTileN] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
+                                                              __uint_as_float(v[4 * q + 2]),
+                                                              __uint_as_float(v[4 * q + 3]));
+                    } else if (OT == AW4_F32 || p.accumulate) {
+                        wg_store_lines<OT, true>(p, stage, first_row, p.n - n + lane, t.k0 + col, v);
+                        wg_store_lines<OT, true>(p, stage, first_row, p.n - n + lane, t.k0 + col + 16, v + 16);
+                    } else {
+                        uint32_t h[16];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q)
+                            h[q] = pack2<OT>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
+                        wg_store_lines<OT, false>(p, stage, first_row, p.n - n + lane, t.k0 + col, h);
                     }
                 }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(smem_addr(&s.acc_empty));
+            if (lane == 0) {
+                bar_arrive(smem_addr(&s.out_done));
+                bar_arrive_cluster(in_first_block(smem_addr(&s.acc_empty)));
+            }
         }
     }
+    // neither block leaves while the other's products or arrivals may reach it
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    pair_sync();
     tc_fence_after();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == kWgProduct) tmem_free(tmem, 512);
     if (threadIdx.x == 0 && s.gave_up && p.status) *reinterpret_cast<volatile int32_t*>(p.status) = 1;
 }
 
 // Adds the parts of each cut tile, in the order of their rows.  Block (b, i): the tile whose first part
-// block b of the main kernel left, rows [16 i, 16 i + 16).
-constexpr int kWgSliceRows = 16;
+// pair b left, rows [32 i, 32 i + 32).
+constexpr int kWgSlice = 32;
 
 template <int OT>
 __global__ void __launch_bounds__(256)
-weight_grad_join_kernel(const WgParams p, int main_blocks) {
+weight_grad_join_kernel(const WgParams p, int pairs) {
     const WgSlot head = p.slots[2 * blockIdx.x + 1];
     if (head.tile < 0) return;
     const WgTile t = wg_tile(p, head.tile);
-    const int row_in = blockIdx.y * kWgSliceRows + threadIdx.x / 16;
-    const int n = t.n0 + row_in;
-    if (n >= p.n) return;
-    float acc[16];
-    const int c0 = threadIdx.x % 16 * 8;       // columns [c0, c0 + 8) and 128 further
-    for (int b = blockIdx.x; b < main_blocks; ++b) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row0 = blockIdx.y * kWgSlice;
+    if (t.n0 + row0 >= p.n) return;
+    __shared__ float tile[kWgSlice][kWgTileK + 4];
+    const bool row_in = t.n0 + row0 + lane < p.n;
+    float4 acc[8] = {};
+    for (int b = blockIdx.x; b < pairs; ++b) {
         const WgSlot slot = b == (int)blockIdx.x ? head : p.slots[2 * b];
         if (slot.tile != head.tile) continue;
-        const float* src = p.partial + ((int64_t)(b == (int)blockIdx.x ? 2 * b + 1 : 2 * b) * kWgTile + row_in) * kWgTile;
+        const int at = b == (int)blockIdx.x ? 2 * b + 1 : 2 * b;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int col = c0 + (h >> 1) * 128 + (h & 1) * 4;
-            const float4 f = t.k0 + col < p.k ? __ldcg(reinterpret_cast<const float4*>(src + col))
-                                              : make_float4(0, 0, 0, 0);
-            const float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[h * 4 + i] = b == (int)blockIdx.x ? v[i] : acc[h * 4 + i] + v[i];
+        for (int q = 0; q < 8; ++q) {
+            const int col = (q * 8 + warp) * 4;
+            if (row_in && t.k0 + col < p.k) {
+                const float4 f = __ldcg(wg_partial(p, at, row0 + lane, col));
+                acc[q].x += f.x;
+                acc[q].y += f.y;
+                acc[q].z += f.z;
+                acc[q].w += f.w;
+            }
         }
         if (slot.ends) break;
     }
-    const int64_t row_off = ((int64_t)t.g * p.n + n) * p.k;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int at = t.k0 + c0 + h * 128;
-        if (at >= p.k) break;
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<float4*>(&tile[lane][(q * 8 + warp) * 4]) = acc[q];
+    __syncthreads();
+    for (int r = warp; r < kWgSlice && t.n0 + row0 + r < p.n; r += 8) {
+        const int64_t row_off = ((int64_t)t.g * p.n + t.n0 + row0 + r) * p.k;
+        const int at = t.k0 + lane * 8;
+        if (at >= p.k) continue;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = tile[r][lane * 8 + i];
         if (p.accumulate) {
             float o[8];
             widen8<OT>(load_raw8<OT>(p.out, row_off, at, p.k, p.vec_out), o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[h * 8 + i] += o[i];
+            for (int i = 0; i < 8; ++i) f[i] += o[i];
         }
-        store_raw8<OT>(p.out, row_off, at, p.k, p.vec_out, narrow8<OT>(acc + h * 8));
+        store_raw8<OT>(p.out, row_off, at, p.k, p.vec_out, narrow8<OT>(f));
     }
 }
 
@@ -518,21 +605,25 @@ static bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, int size, co
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Blocks: one for each tile, more where few tiles have many rows (kWgMinSteps steps a block at least), at
-// most one on each SM.  With groups only their average is known here.
-constexpr int64_t kWgMinSteps = 4;
-
-static int wg_grid(int device, int64_t rows, int64_t n, int64_t k, int64_t groups) {
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 1;
-    const int64_t tiles = (n + kWgTile - 1) / kWgTile * ((k + kWgTile - 1) / kWgTile);
-    const int64_t steps = std::max<int64_t>(groups, (rows + kWgRows - 1) / kWgRows) * tiles;
-    const int64_t want = std::max(tiles * groups, steps / kWgMinSteps);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, sms, kWgMaxBlocks}));
+static int64_t wg_tiles(int64_t n, int64_t k) {
+    return (n + kWgTileN - 1) / kWgTileN * ((k + kWgTileK - 1) / kWgTileK);
 }
 
-static uint64_t wg_workspace(int blocks) {
-    return (uint64_t)blocks * 2 * (sizeof(WgSlot) + (uint64_t)kWgTile * kWgTile * sizeof(float));
+// Pairs of blocks: one for each tile, more where few tiles have many rows (kWgMinSteps steps a pair at
+// least), at most one on each two SMs.  With groups only their average is known here.
+constexpr int64_t kWgMinSteps = 4;
+
+static int wg_pairs(int device, int64_t rows, int64_t n, int64_t k, int64_t groups) {
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 2) sms = 2;
+    const int64_t tiles = wg_tiles(n, k);
+    const int64_t steps = std::max<int64_t>(groups, (rows + kWgRows - 1) / kWgRows) * tiles;
+    const int64_t want = std::max(tiles * groups, steps / kWgMinSteps);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, sms / 2, kWgMaxPairs}));
+}
+
+static uint64_t wg_workspace(int pairs) {
+    return (uint64_t)pairs * 2 * (sizeof(WgSlot) + (uint64_t)kWgTileN * kWgTileK * sizeof(float));
 }
 
 }  // namespace aw4
@@ -541,7 +632,7 @@ using namespace aw4;
 
 extern "C" uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device) {
     if (rows <= 0 || n <= 0 || k <= 0 || groups < 1) return 0;
-    return wg_workspace(wg_grid(device, rows, n, k, groups));
+    return wg_workspace(wg_pairs(device, rows, n, k, groups));
 }
 
 extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
@@ -556,7 +647,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     if (rows < 0 || n < 0 || k < 0 || groups < 1 || (!offsets && groups != 1))
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: bad size");
     if (rows > 0x7fffff00 || n > 1 << 20 || k > 1 << 20 || groups > 65535 ||
-        (n + kWgTile - 1) / kWgTile * ((k + kWgTile - 1) / kWgTile) * groups > 0x7fffff00)
+        wg_tiles(n, k) * groups > 0x7fffff00)
         return fail(AW4_ERR_UNSUPPORTED, "aw4_weight_grad: size above the kernel's");
     if (n == 0 || k == 0) return AW4_OK;
     if (!out || (uintptr_t)out % (out_dtype == AW4_F32 ? 4 : 2))
@@ -571,8 +662,8 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     }
     if (!dy || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)dy % 16 || ld < n || ld * 2 % 16)
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: null buffer, or rows not on 16 bytes");
-    const int grid = wg_grid(device, rows, n, k, groups);
-    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)wg_workspace(grid))
+    const int pairs = wg_pairs(device, rows, n, k, groups);
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)wg_workspace(pairs))
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: workspace of %lld bytes is too small or misaligned",
                     (long long)workspace_bytes);
     if (!encode_tiled()) return fail(AW4_ERR_CUDA, "aw4_weight_grad: the driver has no cuTensorMapEncodeTiled");
@@ -580,8 +671,8 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     p.rows = rows;
     p.n = (int)n;
     p.k = (int)k;
-    p.n_tiles = (int)((n + kWgTile - 1) / kWgTile);
-    p.k_tiles = (int)((k + kWgTile - 1) / kWgTile);
+    p.n_tiles = (int)((n + kWgTileN - 1) / kWgTileN);
+    p.k_tiles = (int)((k + kWgTileK - 1) / kWgTileK);
     p.groups = (int)groups;
     p.blocks = (uint32_t)((k + kA8Block - 1) / kA8Block);
     p.scales = scales;
@@ -590,7 +681,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     p.accumulate = accumulate != 0;
     p.vec_out = (uintptr_t)out % 16 == 0 && k * size % 16 == 0;
     p.partial = static_cast<float*>(workspace);
-    p.slots = reinterpret_cast<WgSlot*>(p.partial + (int64_t)grid * 2 * kWgTile * kWgTile);
+    p.slots = reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK);
     p.status = status;
     CUtensorMap dy_map, code_map;
     if (!encode_rows(&dy_map, dtype == AW4_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
@@ -602,14 +693,14 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
         auto kernel = weight_grad_kernel<dt.value, ot.value>;
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem);
         if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "weight_grad: %s", cudaGetErrorString(e));
-        kernel<<<grid, kWgThreads, kWgSmem, s>>>(dy_map, code_map, p);
+        kernel<<<2 * pairs, kWgThreads, kWgSmem, s>>>(dy_map, code_map, p);
         note_launch();
         e = cudaGetLastError();
         if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "weight_grad launch: %s", cudaGetErrorString(e));
-        // without groups the host knows that blocks with whole tiles leave no parts
+        // without groups the host knows that pairs with whole tiles leave no parts
         const int64_t tiles = (int64_t)p.n_tiles * p.k_tiles;
-        if (!offsets && tiles % grid == 0) return AW4_OK;
-        weight_grad_join_kernel<ot.value><<<dim3(grid, kWgTile / kWgSliceRows), 256, 0, s>>>(p, grid);
+        if (!offsets && tiles % pairs == 0) return AW4_OK;
+        weight_grad_join_kernel<ot.value><<<dim3(pairs, kWgTileN / kWgSlice), 256, 0, s>>>(p, pairs);
         note_launch();
         e = cudaGetLastError();
         return e == cudaSuccess ? AW4_OK : fail(AW4_ERR_CUDA, "weight_grad_join launch: %s", cudaGetErrorString(e));
