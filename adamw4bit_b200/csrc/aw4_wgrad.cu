@@ -9,7 +9,7 @@
 // at a time.  In each block:
 //
 //   warp 16      bulk tensor copies of its dy [64][256] and codes [64][128], four stages
-//   warps 0-15   codes * 2^e -> 16-bit values in shared memory, three buffers, two groups
+//   warps 0-15   codes * 2^e -> 16-bit values in shared memory, four buffers, two groups
 //                of warps taking turns.  A lane owns a block of 32 codes of one row
 //   warp 17      (first block) tcgen05.mma for the pair, both operands with the row
 //                index as the inner dimension
@@ -47,7 +47,7 @@ namespace aw4 {
 
 constexpr int kWgTileN = 512, kWgTileK = 256;   // a pair's tile
 constexpr int kWgRows = 64;                     // rows of a step
-constexpr int kWgStages = 4, kWgBuffers = 3;
+constexpr int kWgStages = 4, kWgBuffers = 4;    // even: see the converting warps
 constexpr int kWgConvert = 512;                 // threads that convert and write out, in two groups
 constexpr int kWgThreads = kWgConvert + 64;
 constexpr int kWgCopy = kWgConvert / 32, kWgProduct = kWgCopy + 1;   // warps
@@ -91,15 +91,16 @@ struct WgShared {
     uint32_t tmem;
     int gave_up;
     int whole;                  // whole tiles of this pair
-    int first_cut, cuts;        // its segments of cut tiles: entries of `list`
+    int first_cut, cuts;        // its cut tiles, and where the first begins and the last ends
+    int first_step, last_step;
     int64_t part[3][kWgThreads / 32];
-    WgSegment list[kWgMaxCut];
 };
 
 constexpr int kWgSmem =
     1024 + kWgStages * (kWgDyBytes + kWgCodeBytes) + kWgBuffers * kWgValBytes + (int)sizeof(WgShared);
 static_assert(kWgSmem <= 227 * 1024, "shared memory of a block");
 static_assert(kWgConvert / 32 * 2048 <= kWgBuffers * kWgValBytes, "2 KB for each warp that writes out");
+static_assert(kWgStages % 2 == 0 && kWgBuffers % 2 == 0, "a stage or buffer belongs to one group of warps");
 static_assert(kWgMaxCut <= kWgThreads, "a thread for each cut tile");
 
 __device__ __forceinline__ void wg_group(const WgParams& p, int g, int64_t& first, int64_t& last) {
@@ -149,8 +150,7 @@ __device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs,
         }
     }
     const int steps = cut + tid < tiles ? wg_steps(p, (cut + tid) / per_group) : 0;
-    if (tid == 0) s.first_cut = kWgMaxCut;
-    if (tid == 1) s.cuts = 0;
+    if (tid == 0) s.cuts = 0;
     const int64_t rest = wg_block_sum(steps, s.part[0]);
     const int64_t target = (wg_block_sum(load, s.part[1]) + rest + pairs - 1) / pairs;
     const int64_t lack = tid < pairs ? max((int64_t)0, target - load) : 0;
@@ -173,9 +173,12 @@ __device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs,
     if (a < b) {
         const int first = (int)(a - at), last = (int)(b - at);
         const int slot = first > 0 ? 2 * pair : last < steps ? 2 * pair + 1 : -1;
-        s.list[tid] = {cut + tid, first, last, slot};
-        atomicMin(&s.first_cut, tid);
         atomicAdd(&s.cuts, 1);
+        if (at <= from) {                              // the pair's first tile
+            s.first_cut = cut + tid;
+            s.first_step = first;
+        }
+        if (at + steps >= to) s.last_step = last;      // its last
         if (writes && slot >= 0) p.slots[slot] = {cut + tid, last == steps};
     }
     if (tid == 0) s.whole = whole;
@@ -183,9 +186,16 @@ __device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs,
 }
 
 __device__ __forceinline__ WgSegment wg_segment(const WgParams& p, const WgShared& s, int i, int pair, int pairs) {
-    if (i >= s.whole) return s.list[s.first_cut + i - s.whole];
-    const int tile = i * pairs + pair;
-    return {tile, 0, wg_steps(p, tile / (p.n_tiles * p.k_tiles)), -1};
+    const bool cut = i >= s.whole;
+    const int c = i - s.whole;
+    const int tile = cut ? s.first_cut + c : i * pairs + pair;
+    const int steps = wg_steps(p, tile / (p.n_tiles * p.k_tiles));
+    WgSegment g = {tile, 0, steps, -1};
+    if (cut && c == 0) g.first = s.first_step;
+    if (cut && c == s.cuts - 1) g.last = s.last_step;
+    if (g.first > 0) g.slot = 2 * pair;
+    else if (g.last < steps) g.slot = 2 * pair + 1;
+    return g;
 }
 
 struct WgTile {
@@ -216,29 +226,65 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+// 2^e twice, in the operand's type; 0 for a row that does not count.
+template <int DT>
+__device__ __forceinline__ uint32_t wg_scale2(int byte, bool live) {
+    uint32_t h;
+    if constexpr (DT == AW4_BF16) {
+        h = byte == kA8Nan ? 0x7fc0u : (uint32_t)byte << 7;
+    } else {
+        const int e = byte - 127;             // down to -24: below -14 a subnormal
+        h = byte == kA8Nan ? 0x7e00u : e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
+    }
+    return live ? h * 0x10001u : 0u;
+}
+
+// q * 2^e of four codes, two and two; every step is exact.
+//   bf16  the code's low seven bits behind 0x43 are 128 + (q mod 128), its sign bit alone 128 or
+//         256: their difference is q
+//   f16   q + 128 behind 0x64 is 1152 + q
+template <int DT>
+__device__ __forceinline__ uint2 wg_values4(uint32_t w, uint32_t s2) {
+    uint2 r;
+    if constexpr (DT == AW4_BF16) {
+        const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t t = __byte_perm(w, 0x43434343u, i ? 0x4342 : 0x4140);
+            const uint32_t x = t & 0xff7fff7fu, y = t & 0xff80ff80u;
+            const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                                     *reinterpret_cast<const __nv_bfloat162*>(&y)), s);
+            (i ? r.y : r.x) = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    } else {
+        const __half2 s = *reinterpret_cast<const __half2*>(&s2);
+        const __half2 off = __float2half2_rn(1152.0f);
+        w ^= 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t t = __byte_perm(w, 0x64646464u, i ? 0x4342 : 0x4140);
+            const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&t), off), s);
+            (i ? r.y : r.x) = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    return r;
+}
+
 // Block j of 32 codes of row r of the step, to 16-bit values.  A quarter of a
 // warp has two rows and four blocks: the order of a block's halves, and the
 // swizzle, put its eight accesses on different banks.
 template <int DT>
-__device__ __forceinline__ void wg_convert(const char* codes, char* operand, int r, int j, int byte, bool live) {
+__device__ __forceinline__ void wg_convert(const char* codes, char* operand, int r, int j, uint32_t s2) {
     char* line = operand + (j >> 1) * kWgBox + r * 128;
     const int swz = r & 7, to = (j & 1) * 4;
-    const float s = a8_scale(byte);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int h = i ^ (j >> 1);
-        uint4 w = *reinterpret_cast<const uint4*>(codes + r * 128 + (((2 * j + h) ^ swz) << 4));
-        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-        uint32_t o[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float v[4];
-            a8_decode4(q[k], s, v);
-            o[2 * k] = live ? pack2<DT>(v[0], v[1]) : 0u;
-            o[2 * k + 1] = live ? pack2<DT>(v[2], v[3]) : 0u;
-        }
-        *reinterpret_cast<uint4*>(line + (((to + 2 * h) ^ swz) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(line + (((to + 2 * h + 1) ^ swz) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        const uint4 w = *reinterpret_cast<const uint4*>(codes + r * 128 + (((2 * j + h) ^ swz) << 4));
+        const uint2 a = wg_values4<DT>(w.x, s2), b = wg_values4<DT>(w.y, s2);
+        const uint2 c = wg_values4<DT>(w.z, s2), d = wg_values4<DT>(w.w, s2);
+        *reinterpret_cast<uint4*>(line + (((to + 2 * h) ^ swz) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<uint4*>(line + (((to + 2 * h + 1) ^ swz) << 4)) = make_uint4(c.x, c.y, d.x, d.y);
     }
 }
 
@@ -420,7 +466,9 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
         }
         __syncwarp();
     } else {
-        const int group = warp >> 3;                   // converts the steps of its parity
+        // Converts the steps of its parity.  Stages and buffers are even in number, so each is of one
+        // group, which sees every turn of its barriers: parity alone tells one turn from the next.
+        const int group = warp >> 3;
         const int r = (warp & 7) * 8 + (lane >> 2), j = lane & 3;
         uint32_t c = 0, buf = 0, turn = 0;
         bool ok = true;
@@ -449,7 +497,9 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                          bar_wait(smem_addr(&s.done[buf]), turn ^ 1, gave_up);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (cols) wg_convert<DT>(code_s + st * kWgCodeBytes, val_s + buf * kWgValBytes, r, j, byte, live);
+                    if (cols)
+                        wg_convert<DT>(code_s + st * kWgCodeBytes, val_s + buf * kWgValBytes, r, j,
+                                       wg_scale2<DT>(byte, live));
                     if (!live) {   // the row belongs to the next group
                         char* line = dy_s + st * kWgDyBytes + j * kWgBox + r * 128;
 #pragma unroll
