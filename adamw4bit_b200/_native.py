@@ -179,7 +179,9 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)   # the same handle without a Stream object
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

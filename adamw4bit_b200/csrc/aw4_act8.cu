@@ -1,8 +1,8 @@
 // aw4_act8.cu -- 8-bit activation checkpoints and the elementwise backward passes that read them.
 //
-// Every kernel here is one pass over its inputs, bound by HBM.  Warps walk
-// runs of kChunks * 32 chunks of eight values; loads of a run are issued
-// before the first is used.
+// Every kernel here is one pass over its inputs, bound by HBM.  A warp takes
+// a run of 32 * k chunks of eight values; the run's loads are issued before the
+// first is used.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -15,83 +15,79 @@ namespace aw4 {
 
 constexpr int kA8Threads = 256;
 constexpr int kChunks = 4;                      // chunks of eight values per lane in flight
-constexpr int kRun = 32 * kChunks;              // chunks per warp and turn
+constexpr int kRun = 32 * kChunks;              // chunks of a warp
 
-// Writes the scale bytes of a run: lane i holds block i's.
+// Writes the scale bytes of a run, 32 blocks, together.
 __device__ __forceinline__ void store_scales(uint8_t* scales, int64_t unit0, int64_t blocks,
-                                             const int b[kChunks], int lane) {
+                                             const A8Block b[kChunks], int lane) {
     int mine = 0;
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-        const int got = __shfl_sync(0xffffffffu, b[j], (lane & 7) * 4);
+        const int got = __shfl_sync(0xffffffffu, b[j].byte, (lane & 7) * 4);
         if ((lane >> 3) == j) mine = got;
     }
     const int64_t blk = (unit0 >> 2) + lane;
     if (blk < blocks) scales[blk] = (uint8_t)mine;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kA8Threads)
-act8_quantize_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t ld, uint32_t per_row,
-                     bool vec, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * (kA8Threads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5); w * kRun < units;
-         w += warps) {
-        const int64_t unit0 = w * kRun;
-        const RunAt run = run_at(unit0, per_row);
-        Raw8<DT> raw[kChunks];
-        bool in[kChunks];
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
-            in[j] = c.in;
-            raw[j] = load_raw8<DT>(x, c.row * ld, c.col, c.in ? cols : 0, vec);
-        }
-        int b[kChunks];
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            float v[8];
-            widen8<DT>(raw[j], v);
-            b[j] = a8_scale_byte<DT>(v);
-            if (in[j])
-                *reinterpret_cast<uint2*>(codes + (unit0 + j * 32 + lane) * 8) = a8_encode8(v, b[j]);
-        }
-        store_scales(scales, unit0, units >> 2, b, lane);
-    }
+// The first chunk of this thread's warp.
+__device__ __forceinline__ int64_t warp_run(int run) {
+    return ((int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5)) * run;
 }
 
 template <int DT>
 __global__ void __launch_bounds__(kA8Threads)
-act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                       int64_t rows, int cols, uint32_t per_row, void* __restrict__ out, int64_t ld,
-                       bool vec) {
+act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, uint8_t* __restrict__ codes,
+                     uint8_t* __restrict__ scales) {
     const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * (kA8Threads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5); w * kRun < units;
-         w += warps) {
-        const int64_t unit0 = w * kRun;
-        const RunAt run = run_at(unit0, per_row);
-        uint2 q[kChunks];
-        int b[kChunks];
+    const int64_t units = rows * per_row, unit0 = warp_run(kRun);
+    if (unit0 >= units) return;
+    const RunAt run = run_at(unit0, per_row);
+    Raw8<DT> raw[kChunks];
+    bool in[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            const int64_t u = unit0 + j * 32 + lane;
-            if (u < units) {
-                q[j] = __ldcs(reinterpret_cast<const uint2*>(codes + u * 8));
-                b[j] = scales[u >> 2];
-            }
-        }
+    for (int j = 0; j < kChunks; ++j) {
+        const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
+        in[j] = c.in;
+        raw[j] = load_raw8<DT>(x, c.in ? c.row : 0, c.col, c.in ? cols : 0);
+    }
+    A8Block b[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
-            if (!c.in) continue;
-            float v[8];
-            a8_decode8(q[j], a8_scale(b[j]), v);
-            store_raw8<DT>(out, c.row * ld, c.col, cols, vec, narrow8<DT>(v));
+    for (int j = 0; j < kChunks; ++j) {
+        float v[8];
+        widen8<DT>(raw[j], v);
+        b[j] = a8_block<DT>(raw[j]);
+        const uint2 q = a8_encode8(v, b[j]);
+        if (in[j]) *reinterpret_cast<uint2*>(codes + (unit0 + j * 32 + lane) * 8) = q;
+    }
+    store_scales(scales, unit0, units >> 2, b, lane);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kA8Threads)
+act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
+                       int cols, uint32_t per_row, const RowsOut out) {
+    const int lane = threadIdx.x & 31;
+    const int64_t units = rows * per_row, unit0 = warp_run(kRun);
+    if (unit0 >= units) return;
+    const RunAt run = run_at(unit0, per_row);
+    uint2 q[kChunks];
+    int b[kChunks];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        const int64_t u = unit0 + j * 32 + lane;
+        if (u < units) {
+            q[j] = __ldcs(reinterpret_cast<const uint2*>(codes + u * 8));
+            b[j] = scales[u >> 2];
         }
+    }
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
+        if (!c.in) continue;
+        float v[8];
+        a8_decode8(q[j], a8_scale(b[j]), v);
+        store_raw8<DT>(out, c.row, c.col, cols, narrow8<DT>(v));
     }
 }
 
@@ -100,116 +96,129 @@ act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restr
 // ---------------------------------------------------------------------------
 
 // exp to a few units in the last place of float32 either way; the 16-bit
-// types take the hardware exponential and reciprocal, far below their rounding.
+// types take the hardware exponential and reciprocal (2^-22 of the value), far below their rounding.
 template <int DT>
 __device__ __forceinline__ float sigmoid(float g) {
-    if constexpr (DT == AW4_F32) return 1.0f / (1.0f + expf(-g));
-    else return __frcp_rn(1.0f + __expf(-g));
+    if constexpr (DT == AW4_F32) {
+        return 1.0f / (1.0f + expf(-g));
+    } else {
+        float e, r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        return r;
+    }
 }
+
+constexpr int kGluChunks = 2, kGluRun = 32 * kGluChunks;
 
 template <int DT, bool EMIT>
 __global__ void __launch_bounds__(kA8Threads)
-swiglu_forward_kernel(const void* __restrict__ gate, const void* __restrict__ up, int64_t rows, int cols,
-                      int64_t ld_gate, int64_t ld_up, uint32_t per_row, bool vec, void* __restrict__ h,
-                      int64_t ld_h, bool vec_h, uint8_t* __restrict__ gcodes, uint8_t* __restrict__ gscales,
+swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols, uint32_t per_row,
+                      const RowsOut h, uint8_t* __restrict__ gcodes, uint8_t* __restrict__ gscales,
                       uint8_t* __restrict__ ucodes, uint8_t* __restrict__ uscales,
                       uint8_t* __restrict__ hcodes, uint8_t* __restrict__ hscales) {
-    constexpr int kC = 2, kR = 32 * kC;
     const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * (kA8Threads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5); w * kR < units; w += warps) {
-        const int64_t unit0 = w * kR;
-        const RunAt run = run_at(unit0, per_row);
-        Raw8<DT> rg[kC], ru[kC];
-        ChunkAt at[kC];
+    const int64_t units = rows * per_row, unit0 = warp_run(kGluRun);
+    if (unit0 >= units) return;
+    const RunAt run = run_at(unit0, per_row);
+    Raw8<DT> rg[kGluChunks], ru[kGluChunks];
+    ChunkAt at[kGluChunks];
 #pragma unroll
-        for (int j = 0; j < kC; ++j) {
-            at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
-            rg[j] = load_raw8<DT>(gate, at[j].row * ld_gate, at[j].col, at[j].in ? cols : 0, vec);
-            ru[j] = load_raw8<DT>(up, at[j].row * ld_up, at[j].col, at[j].in ? cols : 0, vec);
+    for (int j = 0; j < kGluChunks; ++j) {
+        at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
+        rg[j] = load_raw8<DT>(gate, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
+        ru[j] = load_raw8<DT>(up, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kGluChunks; ++j) {
+        const int64_t u = unit0 + j * 32 + lane;
+        float g[8], p[8], y[8];
+        widen8<DT>(rg[j], g);
+        widen8<DT>(ru[j], p);
+        const A8Block bg = a8_block<DT>(rg[j]), bu = a8_block<DT>(ru[j]);
+        const uint2 qg = a8_encode8(g, bg), qu = a8_encode8(p, bu);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = sigmoid<DT>(g[i]);
+        vmul8(y, y, g);
+        vmul8(y, y, p);
+        const Raw8<DT> r = narrow8<DT>(y);
+        A8Block bh = {0, 0.0f};
+        uint2 qh = make_uint2(0, 0);
+        if constexpr (EMIT) {       // the checkpoint of h is that of its rounded values
+            widen8<DT>(r, y);
+            bh = a8_block<DT>(r);
+            qh = a8_encode8(y, bh);
         }
-#pragma unroll
-        for (int j = 0; j < kC; ++j) {
-            const int64_t u = unit0 + j * 32 + lane;
-            float g[8], p[8], y[8];
-            widen8<DT>(rg[j], g);
-            widen8<DT>(ru[j], p);
-            const int bg = a8_scale_byte<DT>(g), bu = a8_scale_byte<DT>(p);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = g[i] * sigmoid<DT>(g[i]) * p[i];
-            const Raw8<DT> r = narrow8<DT>(y);
-            int bh = 0;
-            if constexpr (EMIT) {       // the checkpoint of h is that of its rounded values
-                widen8<DT>(r, y);
-                bh = a8_scale_byte<DT>(y);
-            }
-            if (at[j].in) {
-                *reinterpret_cast<uint2*>(gcodes + u * 8) = a8_encode8(g, bg);
-                *reinterpret_cast<uint2*>(ucodes + u * 8) = a8_encode8(p, bu);
-                store_raw8<DT>(h, at[j].row * ld_h, at[j].col, cols, vec_h, r);
-                if constexpr (EMIT) *reinterpret_cast<uint2*>(hcodes + u * 8) = a8_encode8(y, bh);
-                if ((lane & 3) == 0) {
-                    gscales[u >> 2] = (uint8_t)bg;
-                    uscales[u >> 2] = (uint8_t)bu;
-                    if constexpr (EMIT) hscales[u >> 2] = (uint8_t)bh;
-                }
-            }
+        if (!at[j].in) continue;
+        *reinterpret_cast<uint2*>(gcodes + u * 8) = qg;
+        *reinterpret_cast<uint2*>(ucodes + u * 8) = qu;
+        store_raw8<DT>(h, at[j].row, at[j].col, cols, r);
+        if constexpr (EMIT) *reinterpret_cast<uint2*>(hcodes + u * 8) = qh;
+        if ((lane & 3) == 0) {
+            gscales[u >> 2] = (uint8_t)bg.byte;
+            uscales[u >> 2] = (uint8_t)bu.byte;
+            if constexpr (EMIT) hscales[u >> 2] = (uint8_t)bh.byte;
         }
     }
 }
 
+// dg = dh u (s + g s (1 - s)), du = dh g s, s = sigmoid(g)
 template <int DT>
 __global__ void __launch_bounds__(kA8Threads)
-swiglu_backward_kernel(const void* __restrict__ dh, int64_t rows, int cols, int64_t ld_dh, uint32_t per_row,
-                       bool vec, const uint8_t* __restrict__ gcodes, const uint8_t* __restrict__ gscales,
+swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row,
+                       const uint8_t* __restrict__ gcodes, const uint8_t* __restrict__ gscales,
                        const uint8_t* __restrict__ ucodes, const uint8_t* __restrict__ uscales,
-                       void* __restrict__ dgate, void* __restrict__ dup, int64_t ld_out, bool vec_out) {
-    constexpr int kC = 2, kR = 32 * kC;
+                       const RowsOut dgate, const RowsOut dup) {
     const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * (kA8Threads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5); w * kR < units; w += warps) {
-        const int64_t unit0 = w * kR;
-        const RunAt run = run_at(unit0, per_row);
-        Raw8<DT> rd[kC];
-        uint2 qg[kC], qu[kC];
-        int bg[kC], bu[kC];
-        ChunkAt at[kC];
+    const int64_t units = rows * per_row, unit0 = warp_run(kGluRun);
+    if (unit0 >= units) return;
+    const RunAt run = run_at(unit0, per_row);
+    Raw8<DT> rd[kGluChunks];
+    uint2 qg[kGluChunks], qu[kGluChunks];
+    int bg[kGluChunks], bu[kGluChunks];
+    ChunkAt at[kGluChunks];
 #pragma unroll
-        for (int j = 0; j < kC; ++j) {
-            const int64_t u = unit0 + j * 32 + lane;
-            at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
-            if (!at[j].in) continue;
-            rd[j] = load_raw8<DT>(dh, at[j].row * ld_dh, at[j].col, cols, vec);
-            qg[j] = __ldcs(reinterpret_cast<const uint2*>(gcodes + u * 8));
-            qu[j] = __ldcs(reinterpret_cast<const uint2*>(ucodes + u * 8));
-            bg[j] = gscales[u >> 2];
-            bu[j] = uscales[u >> 2];
+    for (int j = 0; j < kGluChunks; ++j) {
+        const int64_t u = unit0 + j * 32 + lane;
+        at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
+        if (!at[j].in) continue;
+        rd[j] = load_raw8<DT>(dh, at[j].row, at[j].col, cols);
+        qg[j] = __ldcs(reinterpret_cast<const uint2*>(gcodes + u * 8));
+        qu[j] = __ldcs(reinterpret_cast<const uint2*>(ucodes + u * 8));
+        bg[j] = gscales[u >> 2];
+        bu[j] = uscales[u >> 2];
+    }
+#pragma unroll
+    for (int j = 0; j < kGluChunks; ++j) {
+        if (!at[j].in) continue;
+        float d[8], g[8], p[8], s[8], f[8];
+        widen8<DT>(rd[j], d);
+        a8_decode8(qg[j], a8_scale(bg[j]), g);
+        a8_decode8(qu[j], a8_scale(bu[j]), p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[i] = sigmoid<DT>(g[i]);
+            f[i] = 1.0f - s[i];
         }
+        vmul8(g, g, s);
 #pragma unroll
-        for (int j = 0; j < kC; ++j) {
-            if (!at[j].in) continue;
-            float d[8], g[8], p[8];
-            widen8<DT>(rd[j], d);
-            a8_decode8(qg[j], a8_scale(bg[j]), g);
-            a8_decode8(qu[j], a8_scale(bu[j]), p);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float s = sigmoid<DT>(g[i]);
-                const float gs = g[i] * s;
-                p[i] = d[i] * p[i] * __fmaf_rn(gs, 1.0f - s, s);
-                g[i] = d[i] * gs;
-            }
-            store_raw8<DT>(dgate, at[j].row * ld_out, at[j].col, cols, vec_out, narrow8<DT>(p));
-            store_raw8<DT>(dup, at[j].row * ld_out, at[j].col, cols, vec_out, narrow8<DT>(g));
-        }
+        for (int i = 0; i < 8; ++i) s[i] = __fmaf_rn(g[i], f[i], s[i]);
+        vmul8(p, p, d);
+        vmul8(p, p, s);
+        vmul8(g, g, d);
+        store_raw8<DT>(dgate, at[j].row, at[j].col, cols, narrow8<DT>(p));
+        store_raw8<DT>(dup, at[j].row, at[j].col, cols, narrow8<DT>(g));
     }
 }
 
 // ---------------------------------------------------------------------------
 // RMS norm: y = x r w, r = (mean(x^2) + eps)^-1/2
 // ---------------------------------------------------------------------------
+//
+// A row belongs to NT threads that hold V chunks of eight values each; NT = 32:
+// a warp a row, no barrier.  Blocks stay and walk the rows, the next row's loads on
+// their way while one is worked on: the weight is read once a block, and the
+// backward kernel keeps its columns' sum of dy v r in registers over all its rows.
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -217,10 +226,10 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Sum over the NT threads that share a row; NT == 32: a warp per row.
-// `slot` alternates so that one barrier per sum is enough.
+// Sum over the NT threads that share a row.  `slot` alternates so that one
+// barrier per sum is enough.
 template <int NT>
-__device__ __forceinline__ float row_sum(float v, float (*part)[32], int slot) {
+__device__ __forceinline__ float row_sum(float v, float (*part)[NT / 32], int slot) {
     v = warp_sum(v);
     if constexpr (NT == 32) {
         return v;
@@ -234,137 +243,191 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[32], int slot) {
     }
 }
 
-__device__ __forceinline__ float load_weight(const void* w, int dtype, int col, int cols) {
-    if (col >= cols) return 0.0f;
-    if (dtype == AW4_F32) return Elem<AW4_F32>::load1(w, col);
-    if (dtype == AW4_BF16) return Elem<AW4_BF16>::load1(w, col);
-    return Elem<AW4_F16>::load1(w, col);
+__device__ __forceinline__ void load_weight8(const void* w, int dtype, int col, int cols, float v[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = 0.0f;
+        if (col + i < cols)
+            v[i] = dtype == AW4_F32    ? Elem<AW4_F32>::load1(w, col + i)
+                   : dtype == AW4_BF16 ? Elem<AW4_BF16>::load1(w, col + i)
+                                       : Elem<AW4_F16>::load1(w, col + i);
+    }
 }
 
-// A row belongs to NT threads that hold V chunks of eight values each.
+template <int NT, int V>
+constexpr int kNormBlocks = V > 1 ? 1 : NT == 32 ? 4 : 1024 / NT;      // resident on an SM
+
 template <int DT, int NT, int V>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
-rms_norm_forward_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t ld, uint32_t per_row,
-                        bool vec, const void* __restrict__ w, int w_dtype, float eps, void* __restrict__ y,
-                        bool vec_y, float* __restrict__ rstd, uint8_t* __restrict__ codes,
-                        uint8_t* __restrict__ scales, uint8_t* __restrict__ ycodes,
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, kNormBlocks<NT, V>)
+rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, const void* __restrict__ w,
+                        int w_dtype, float eps, const RowsOut y, float* __restrict__ rstd,
+                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ ycodes,
                         uint8_t* __restrict__ yscales) {
-    __shared__ float part[2][32];
-    constexpr int kRows = NT == 32 ? 8 : 1;
+    __shared__ float part[2][NT / 32];
+    const int held = NT == 32 ? blockDim.x >> 5 : 1;       // rows of a block at a time
     const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + (NT == 32 ? threadIdx.x >> 5 : 0); row < rows;
-         row += (int64_t)gridDim.x * kRows, slot ^= 1) {
-        Raw8<DT> raw[V];
+    const int64_t step = (int64_t)gridDim.x * held;
+    int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
+    float wv[V][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT>(x, row * ld, (j * NT + t) * 8, cols, vec);
-        float ss = 0.0f;
+    for (int j = 0; j < V; ++j) load_weight8(w, w_dtype, (j * NT + t) * 8, cols, wv[j]);
+    Raw8<DT> raw[V];
+    if (row < rows)
+#pragma unroll
+        for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT>(x, row, (j * NT + t) * 8, cols);
+    for (int slot = 0; row < rows; row += step, slot ^= 1) {
+        Raw8<DT> next[V];
+        if (row + step < rows)
+#pragma unroll
+            for (int j = 0; j < V; ++j) next[j] = load_raw8<DT>(x, row + step, (j * NT + t) * 8, cols);
+        f2 ss = pk2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float v[8];
             widen8<DT>(raw[j], v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = __fmaf_rn(v[i], v[i], ss);
+            for (int i = 0; i < 8; i += 2) ss = f2_fma(pk2(v[i], v[i + 1]), pk2(v[i], v[i + 1]), ss);
         }
-        const float r = 1.0f / sqrtf(row_sum<NT>(ss, part, slot) / (float)cols + eps);
+        float s0, s1;
+        upk2(ss, s0, s1);
+        const float r = 1.0f / sqrtf(row_sum<NT>(s0 + s1, part, slot) / (float)cols + eps);
         if (t == 0) rstd[row] = r;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t u = j * NT + t;
-            const int col = (int)u * 8;
             float v[8], o[8];
             widen8<DT>(raw[j], v);
-            const int b = a8_scale_byte<DT>(v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = v[i] * r * load_weight(w, w_dtype, col + i, cols);
+            const A8Block b = a8_block<DT>(raw[j]);
+            const uint2 q = a8_encode8(v, b);
+            vmuls8(o, v, r);
+            vmul8(o, o, wv[j]);
             const Raw8<DT> ry = narrow8<DT>(o);
-            int by = 0;
+            A8Block by = {0, 0.0f};
+            uint2 qy = make_uint2(0, 0);
             if (ycodes) {               // the checkpoint of y is that of its rounded values
                 widen8<DT>(ry, o);
-                by = a8_scale_byte<DT>(o);
+                by = a8_block<DT>(ry);
+                qy = a8_encode8(o, by);
             }
             if (u < per_row) {
                 const int64_t at = row * per_row + u;
-                *reinterpret_cast<uint2*>(codes + at * 8) = a8_encode8(v, b);
-                if ((t & 3) == 0) scales[at >> 2] = (uint8_t)b;
-                store_raw8<DT>(y, row * cols, col, cols, vec_y, ry);
+                *reinterpret_cast<uint2*>(codes + at * 8) = q;
+                if ((t & 3) == 0) scales[at >> 2] = (uint8_t)b.byte;
+                store_raw8<DT>(y, row, (int)u * 8, cols, ry);
                 if (ycodes) {
-                    *reinterpret_cast<uint2*>(ycodes + at * 8) = a8_encode8(o, by);
-                    if ((t & 3) == 0) yscales[at >> 2] = (uint8_t)by;
+                    *reinterpret_cast<uint2*>(ycodes + at * 8) = qy;
+                    if ((t & 3) == 0) yscales[at >> 2] = (uint8_t)by.byte;
                 }
             }
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) raw[j] = next[j];
     }
+}
+
+// What a thread has of a row of the backward pass.
+template <int DT, int V>
+struct NormRow {
+    Raw8<DT> dy[V];
+    uint2 q[V];
+    int b[V];
+    float r;
+};
+
+template <int DT, int NT, int V>
+__device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& dy, int64_t row, int t, int cols,
+                                              uint32_t per_row, const uint8_t* codes, const uint8_t* scales,
+                                              const float* rstd) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const uint32_t u = j * NT + t;
+        const int64_t at = row * per_row + u;
+        n.dy[j] = load_raw8<DT>(dy, row, (int)u * 8, cols);
+        n.q[j] = make_uint2(0, 0);
+        n.b[j] = 1;
+        if (u < per_row) {
+            n.q[j] = __ldcs(reinterpret_cast<const uint2*>(codes + at * 8));
+            n.b[j] = scales[at >> 2];
+        }
+    }
+    n.r = rstd[row];
 }
 
 // dx = r (w dy) - v r^3 mean(v w dy); each block leaves its rows' sum of
 // dy v r in partial[blockIdx.x][cols].
 template <int DT, int NT, int V>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
-rms_norm_backward_kernel(const void* __restrict__ dy, int64_t rows, int cols, int64_t ld, uint32_t per_row,
-                         bool vec, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, kNormBlocks<NT, V>)
+rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, uint32_t per_row,
+                         const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                          const float* __restrict__ rstd, const void* __restrict__ w, int w_dtype,
-                         void* __restrict__ dx, bool vec_dx, float* __restrict__ partial) {
-    __shared__ float part[2][32];
-    constexpr int kRows = NT == 32 ? 8 : 1;
+                         const RowsOut dx, float* __restrict__ partial) {
+    __shared__ float part[2][NT / 32];
+    const int held = NT == 32 ? blockDim.x >> 5 : 1;
     const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    float acc[V][8] = {};
-    int slot = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + (NT == 32 ? threadIdx.x >> 5 : 0); row < rows;
-         row += (int64_t)gridDim.x * kRows, slot ^= 1) {
-        Raw8<DT> raw[V];
-        uint2 q[V];
-        int b[V];
+    const int64_t step = (int64_t)gridDim.x * held;
+    int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
+    float wv[V][8], acc[V][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t u = j * NT + t;
-            const int64_t at = row * per_row + u;
-            raw[j] = load_raw8<DT>(dy, row * ld, (int)u * 8, cols, vec);
-            q[j] = u < per_row ? __ldcs(reinterpret_cast<const uint2*>(codes + at * 8)) : make_uint2(0, 0);
-            b[j] = u < per_row ? scales[at >> 2] : 1;
-        }
-        const float r = rstd[row];
-        float dot = 0.0f;
+    for (int j = 0; j < V; ++j) {
+        load_weight8(w, w_dtype, (j * NT + t) * 8, cols, wv[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
+    }
+    NormRow<DT, V> now;
+    if (row < rows) load_norm_row<DT, NT, V>(now, dy, row, t, cols, per_row, codes, scales, rstd);
+    for (int slot = 0; row < rows; row += step, slot ^= 1) {
+        NormRow<DT, V> next;
+        if (row + step < rows)
+            load_norm_row<DT, NT, V>(next, dy, row + step, t, cols, per_row, codes, scales, rstd);
+        const float r = now.r;
+        f2 dot2 = pk2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float d[8], v[8];
-            widen8<DT>(raw[j], d);
-            a8_decode8(q[j], a8_scale(b[j]), v);
+            widen8<DT>(now.dy[j], d);
+            a8_decode8(now.q[j], a8_scale(now.b[j]), v);
+            vmul8(d, d, v);
+            // behind the last column codes and gradients are zero, but a block may be NaN
+            if ((int)(j * NT + t) * 8 + 8 > cols)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int col = (j * NT + t) * 8 + i;
-                const float dv = col < cols ? d[i] * v[i] : 0.0f;
-                dot = __fmaf_rn(dv, load_weight(w, w_dtype, col, cols), dot);
-                acc[j][i] = __fmaf_rn(dv, r, acc[j][i]);
-            }
+                for (int i = 0; i < 8; ++i)
+                    if ((int)(j * NT + t) * 8 + i >= cols) d[i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+                dot2 = f2_fma(pk2(d[i], d[i + 1]), pk2(wv[j][i], wv[j][i + 1]), dot2);
+            vfmas8(acc[j], r, d, acc[j]);
         }
-        const float k = r * r * r * (row_sum<NT>(dot, part, slot) / (float)cols);
+        float d0, d1;
+        upk2(dot2, d0, d1);
+        const float k = r * r * r * (row_sum<NT>(d0 + d1, part, slot) / (float)cols);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t u = j * NT + t;
             float d[8], v[8];
-            widen8<DT>(raw[j], d);
-            a8_decode8(q[j], a8_scale(b[j]), v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                d[i] = __fmaf_rn(r * load_weight(w, w_dtype, (int)u * 8 + i, cols), d[i], -(v[i] * k));
-            if (u < per_row) store_raw8<DT>(dx, row * cols, (int)u * 8, cols, vec_dx, narrow8<DT>(d));
+            widen8<DT>(now.dy[j], d);
+            a8_decode8(now.q[j], a8_scale(now.b[j]), v);
+            vmul8(d, d, wv[j]);
+            vmuls8(d, d, r);
+            vfmas8(d, -k, v, d);
+            if (u < per_row) store_raw8<DT>(dx, row, (int)u * 8, cols, narrow8<DT>(d));
         }
+        now = next;
     }
     if constexpr (NT == 32) {
-        // the block's eight warps hold the same columns: added in their order
+        // the block's warps hold the same columns: added in their order
         __shared__ float sums[V * 256];
-        for (int i = threadIdx.x; i < V * 256; i += 256) sums[i] = 0.0f;
-        for (int wi = 0; wi < 8; ++wi) {
-            __syncthreads();
+        for (int wi = 0; wi < held; ++wi) {
             if ((int)(threadIdx.x >> 5) == wi)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sums[(j * 32 + t) * 8 + i] += acc[j][i];
+                    for (int i = 0; i < 8; ++i) {
+                        float& s = sums[(j * 32 + t) * 8 + i];
+                        s = wi ? s + acc[j][i] : acc[j][i];
+                    }
+            __syncthreads();
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < cols; i += 256) partial[(int64_t)blockIdx.x * cols + i] = sums[i];
+        for (int i = threadIdx.x; i < cols; i += blockDim.x) partial[(int64_t)blockIdx.x * cols + i] = sums[i];
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -384,6 +447,7 @@ column_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* 
     const int c = blockIdx.x * 32 + threadIdx.x;
     float v = 0.0f;
     if (c < cols)
+#pragma unroll 8
         for (int p = threadIdx.y; p < parts; p += 32) v += partial[(int64_t)p * cols + c];
     s[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
@@ -395,13 +459,6 @@ column_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-
-static int sm_count(int device) {
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0)
-        sms = 1;
-    return sms;
-}
 
 static bool known_dtype(int dtype) { return dtype >= AW4_F32 && dtype <= AW4_F16; }
 static int size_of(int dtype) { return dtype == AW4_F32 ? 4 : 2; }
@@ -415,6 +472,8 @@ static int32_t check_matrix(const char* what, int dtype, int64_t rows, int64_t c
     if (!known_dtype(dtype)) return fail(AW4_ERR_INVALID, "%s: bad dtype %d", what, dtype);
     if (rows < 0 || cols < 0) return fail(AW4_ERR_INVALID, "%s: negative size", what);
     if (cols > (int64_t)1 << 30) return fail(AW4_ERR_UNSUPPORTED, "%s: rows of more than 2^30 values", what);
+    if (rows && cols > ((int64_t)1 << 40) / rows)
+        return fail(AW4_ERR_UNSUPPORTED, "%s: more than 2^40 values", what);
     return AW4_OK;
 }
 
@@ -426,23 +485,29 @@ static int32_t launched(const char* what) {
 
 static uint32_t chunks_per_row(int64_t cols) { return (uint32_t)((cols + kA8Block - 1) / kA8Block * 4); }
 
-static int run_grid(int device, int64_t units, int run) {
+static unsigned run_grid(int64_t units, int run) {
     const int64_t per_block = (int64_t)run * (kA8Threads / 32);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((units + per_block - 1) / per_block,
-                                                       (int64_t)sm_count(device) * 64));
+    return (unsigned)((units + per_block - 1) / per_block);
 }
 
-// Rows' threads and chunks: the fewest threads whose chunks cover the row.
-// Up to 1024 columns a warp holds a row and needs no barrier.
+static RowsIn rows_in(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+    const char* base = static_cast<const char*>(p);
+    return {base, base + ((rows - 1) * ld + cols) * size_of(dtype), ld, vec_ok(p, ld, dtype)};
+}
+static RowsOut rows_out(void* p, int64_t ld, int dtype) { return {static_cast<char*>(p), ld, vec_ok(p, ld, dtype)}; }
+
+// A row's threads and chunks: one chunk a thread where 512 threads cover the row (the sums and weights of two
+// chunks take the registers of half the warps), a warp without a barrier up to 256 columns.
 template <typename F>
 static int32_t norm_shape(int64_t cols, F f) {
-    if (cols <= 256) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
-    if (cols <= 512) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 2>());
-    if (cols <= 1024) return f(std::integral_constant<int, 32>(), std::integral_constant<int, 4>());
-    if (cols <= 2048) return f(std::integral_constant<int, 128>(), std::integral_constant<int, 2>());
-    if (cols <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    if (cols <= 8192) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
-    return f(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+    using std::integral_constant;
+    if (cols <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
+    if (cols <= 512) return f(integral_constant<int, 64>(), integral_constant<int, 1>());
+    if (cols <= 1024) return f(integral_constant<int, 128>(), integral_constant<int, 1>());
+    if (cols <= 2048) return f(integral_constant<int, 256>(), integral_constant<int, 1>());
+    if (cols <= 4096) return f(integral_constant<int, 512>(), integral_constant<int, 1>());
+    if (cols <= 8192) return f(integral_constant<int, 512>(), integral_constant<int, 2>());
+    return f(integral_constant<int, 1024>(), integral_constant<int, 2>());
 }
 
 template <typename F>
@@ -454,12 +519,17 @@ static int32_t by_dtype(int dtype, F f) {
 
 constexpr int64_t kNormCols = 16384;
 
-// Blocks of the backward kernel, and so rows of its partial sums.
-static int norm_backward_grid(int device, int64_t rows, int64_t cols) {
-    const int64_t per_block = cols <= 1024 ? 8 : 1;
-    const int per_sm = cols <= 2048 ? 4 : cols <= 4096 ? 3 : 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per_block - 1) / per_block,
-                                                       (int64_t)sm_count(device) * per_sm));
+// Where a warp has a row: warps of a block, one for each SM's share of few rows, eight at most.
+static int norm_warps(int device, int64_t rows) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(8, rows / sm_count(device)));
+}
+
+// Resident blocks, or as many as have a row: of the backward kernel also the rows of its partial sums.
+template <int NT, int V>
+static int norm_grid(int device, int64_t rows) {
+    const int held = NT == 32 ? norm_warps(device, rows) : 1;
+    const int resident = NT == 32 ? kNormBlocks<NT, V> * 8 / held : kNormBlocks<NT, V>;
+    return (int)std::min<int64_t>((rows + held - 1) / held, (int64_t)sm_count(device) * resident);
 }
 
 }  // namespace aw4
@@ -476,9 +546,8 @@ extern "C" int32_t aw4_act8_quantize(const void* x, int32_t dtype, int64_t rows,
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
-        act8_quantize_kernel<dt.value><<<run_grid(device, rows * per_row, kRun), kA8Threads, 0,
-                                         (cudaStream_t)stream>>>(x, rows, (int)cols, ld, per_row,
-                                                                 vec_ok(x, ld, dtype), codes, scales);
+        act8_quantize_kernel<dt.value><<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(
+            rows_in(x, rows, cols, ld, dtype), rows, (int)cols, per_row, codes, scales);
         return launched("act8_quantize");
     });
 }
@@ -494,9 +563,8 @@ extern "C" int32_t aw4_act8_dequantize(const uint8_t* codes, const uint8_t* scal
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
-        act8_dequantize_kernel<dt.value><<<run_grid(device, rows * per_row, kRun), kA8Threads, 0,
-                                           (cudaStream_t)stream>>>(codes, scales, rows, (int)cols, per_row,
-                                                                   out, ld, vec_ok(out, ld, dtype));
+        act8_dequantize_kernel<dt.value><<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(
+            codes, scales, rows, (int)cols, per_row, rows_out(out, ld, dtype));
         return launched("act8_dequantize");
     });
 }
@@ -513,17 +581,16 @@ extern "C" int32_t aw4_swiglu_forward(const void* gate, const void* up, int32_t 
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
-    const bool vec = vec_ok(gate, ld_gate, dtype) && vec_ok(up, ld_up, dtype);
-    const int grid = run_grid(device, rows * per_row, 64);
+    const RowsIn g = rows_in(gate, rows, cols, ld_gate, dtype), u = rows_in(up, rows, cols, ld_up, dtype);
+    const RowsOut o = rows_out(h, cols, dtype);
+    const unsigned grid = run_grid(rows * per_row, kGluRun);
     return by_dtype(dtype, [&](auto dt) {
         if (hcodes)
             swiglu_forward_kernel<dt.value, true><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
-                gate, up, rows, (int)cols, ld_gate, ld_up, per_row, vec, h, cols, vec_ok(h, cols, dtype),
-                gcodes, gscales, ucodes, uscales, hcodes, hscales);
+                g, u, rows, (int)cols, per_row, o, gcodes, gscales, ucodes, uscales, hcodes, hscales);
         else
             swiglu_forward_kernel<dt.value, false><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
-                gate, up, rows, (int)cols, ld_gate, ld_up, per_row, vec, h, cols, vec_ok(h, cols, dtype),
-                gcodes, gscales, ucodes, uscales, nullptr, nullptr);
+                g, u, rows, (int)cols, per_row, o, gcodes, gscales, ucodes, uscales, nullptr, nullptr);
         return launched("swiglu_forward");
     });
 }
@@ -541,10 +608,10 @@ extern "C" int32_t aw4_swiglu_backward(const void* dh, int32_t dtype, int64_t ro
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
-        swiglu_backward_kernel<dt.value><<<run_grid(device, rows * per_row, 64), kA8Threads, 0,
-                                           (cudaStream_t)stream>>>(
-            dh, rows, (int)cols, ld_dh, per_row, vec_ok(dh, ld_dh, dtype), gcodes, gscales, ucodes, uscales,
-            dgate, dup, ld_out, vec_ok(dgate, ld_out, dtype) && vec_ok(dup, ld_out, dtype));
+        swiglu_backward_kernel<dt.value>
+            <<<run_grid(rows * per_row, kGluRun), kA8Threads, 0, (cudaStream_t)stream>>>(
+                rows_in(dh, rows, cols, ld_dh, dtype), rows, (int)cols, per_row, gcodes, gscales, ucodes, uscales,
+                rows_out(dgate, ld_out, dtype), rows_out(dup, ld_out, dtype));
         return launched("swiglu_backward");
     });
 }
@@ -567,12 +634,11 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
         return norm_shape(cols, [&](auto nt, auto v) {
-            constexpr int kRows = nt.value == 32 ? 8 : 1;
-            const int grid = (int)std::min<int64_t>((rows + kRows - 1) / kRows, (int64_t)sm_count(device) * 64);
             rms_norm_forward_kernel<dt.value, nt.value, v.value>
-                <<<grid, nt.value == 32 ? 256 : nt.value, 0, (cudaStream_t)stream>>>(
-                    x, rows, (int)cols, ld, per_row, vec_ok(x, ld, dtype), weight, weight_dtype, eps, y,
-                    vec_ok(y, cols, dtype), rstd, codes, scales, ycodes, yscales);
+                <<<norm_grid<nt.value, v.value>(device, rows),
+                   nt.value == 32 ? 32 * norm_warps(device, rows) : nt.value, 0, (cudaStream_t)stream>>>(
+                    rows_in(x, rows, cols, ld, dtype), rows, (int)cols, per_row, weight, weight_dtype, eps,
+                    rows_out(y, cols, dtype), rstd, codes, scales, ycodes, yscales);
             return launched("rms_norm_forward");
         });
     });
@@ -580,7 +646,12 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
 
 extern "C" uint64_t aw4_rms_norm_backward_workspace(int64_t rows, int64_t cols, int32_t device) {
     if (rows <= 0 || cols <= 0 || cols > kNormCols) return 0;
-    return (uint64_t)norm_backward_grid(device, rows, cols) * cols * sizeof(float);
+    int grid = 0;
+    norm_shape(cols, [&](auto nt, auto v) {
+        grid = norm_grid<nt.value, v.value>(device, rows);
+        return AW4_OK;
+    });
+    return (uint64_t)grid * cols * sizeof(float);
 }
 
 extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
@@ -605,17 +676,18 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
     }
     if (!dy || !codes || !scales || !rstd || !weight || !dx || (uintptr_t)codes % 16)
         return fail(AW4_ERR_INVALID, "aw4_rms_norm_backward: null or misaligned buffer");
-    const int grid = norm_backward_grid(device, rows, cols);
-    if (!workspace || workspace_bytes < (int64_t)grid * cols * (int64_t)sizeof(float))
+    if (!workspace || workspace_bytes < (int64_t)aw4_rms_norm_backward_workspace(rows, cols, device))
         return fail(AW4_ERR_INVALID, "aw4_rms_norm_backward: workspace of %lld bytes is too small",
                     (long long)workspace_bytes);
     const uint32_t per_row = chunks_per_row(cols);
+    int grid = 0;
     const int32_t rc = by_dtype(dtype, [&](auto dt) {
         return norm_shape(cols, [&](auto nt, auto v) {
+            grid = norm_grid<nt.value, v.value>(device, rows);
             rms_norm_backward_kernel<dt.value, nt.value, v.value>
-                <<<grid, nt.value == 32 ? 256 : nt.value, 0, s>>>(
-                    dy, rows, (int)cols, ld, per_row, vec_ok(dy, ld, dtype), codes, scales, rstd, weight,
-                    weight_dtype, dx, vec_ok(dx, cols, dtype), workspace);
+                <<<grid, nt.value == 32 ? 32 * norm_warps(device, rows) : nt.value, 0, s>>>(
+                    rows_in(dy, rows, cols, ld, dtype), rows, (int)cols, per_row, codes, scales, rstd, weight,
+                    weight_dtype, rows_out(dx, cols, dtype), workspace);
             return launched("rms_norm_backward");
         });
     });

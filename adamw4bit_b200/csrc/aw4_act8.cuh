@@ -35,34 +35,117 @@ struct Raw8 {
     uint4 w[Elem<DT>::kBytes / 2];
 };
 
-// Values [col, col + 8) of a row at `base`; zeros from `cols` on.  `vec`: the
-// row starts on 16 bytes, so that whole chunks are vector loads.
+// Rows of a matrix in memory.  `vec`: every row starts on 16 bytes.
+struct RowsIn {
+    const char* base;
+    const char* end;      // behind the last value
+    int64_t ld;           // values from row to row
+    bool vec;
+};
+struct RowsOut {
+    char* base;
+    int64_t ld;
+    bool vec;
+};
+
+// Values [col, col + 8) of a row; zeros from `cols` on.
 template <int DT>
-__device__ __forceinline__ Raw8<DT> load_raw8(const void* base, int64_t row_off, int col, int cols,
-                                              bool vec) {
+__device__ __forceinline__ Raw8<DT> load_raw8(const RowsIn& m, int64_t row, int col, int cols) {
+    constexpr int kSize = Elem<DT>::kBytes, kWords = kSize * 2;
     Raw8<DT> r;
-    if (vec && col + 8 <= cols) {
-        const char* p = static_cast<const char*>(base) + (row_off + col) * Elem<DT>::kBytes;
+    uint32_t* w = reinterpret_cast<uint32_t*>(r.w);
+    const char* p = m.base + (row * m.ld + col) * kSize;
+    if (col + 8 <= cols) {
+        if (m.vec) {
 #pragma unroll
-        for (int i = 0; i < Elem<DT>::kBytes / 2; ++i)
-            r.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+            for (int i = 0; i < kSize / 2; ++i) r.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+            return r;
+        }
+        // the aligned words around them, where those lie inside the matrix, shifted into place
+        const char* q = reinterpret_cast<const char*>((uintptr_t)p & ~(uintptr_t)15);
+        constexpr int kLoads = kSize / 2 + 1;
+        if (q >= m.base && q + 16 * kLoads <= m.end) {
+            uint32_t v[4 * kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(q) + i);
+            const uint32_t at = (uint32_t)(p - q);
+            if (at & 8)
+#pragma unroll
+                for (int i = 0; i + 2 < 4 * kLoads; ++i) v[i] = v[i + 2];
+            if (at & 4)
+#pragma unroll
+                for (int i = 0; i + 1 < 4 * kLoads; ++i) v[i] = v[i + 1];
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                w[i] = kSize == 2 && (at & 2) ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
+            return r;
+        }
+    }
+    if constexpr (DT == AW4_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = col + i < cols ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
     } else {
-        uint32_t* w = reinterpret_cast<uint32_t*>(r.w);
-        if constexpr (DT == AW4_F32) {
-            const uint32_t* p = static_cast<const uint32_t*>(base) + row_off;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = col + i < cols ? p[col + i] : 0u;
-        } else {
-            const uint16_t* p = static_cast<const uint16_t*>(base) + row_off;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t lo = col + 2 * i < cols ? p[col + 2 * i] : 0u;
-                const uint32_t hi = col + 2 * i + 1 < cols ? p[col + 2 * i + 1] : 0u;
-                w[i] = lo | (hi << 16);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = col + 2 * i < cols ? reinterpret_cast<const uint16_t*>(p)[2 * i] : 0u;
+            const uint32_t hi = col + 2 * i + 1 < cols ? reinterpret_cast<const uint16_t*>(p)[2 * i + 1] : 0u;
+            w[i] = lo | (hi << 16);
         }
     }
     return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void store_raw8(const RowsOut& m, int64_t row, int col, int cols, const Raw8<DT>& r) {
+    constexpr int kSize = Elem<DT>::kBytes;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+    char* p = m.base + (row * m.ld + col) * kSize;
+    if (col + 8 <= cols) {
+        if (m.vec) {
+#pragma unroll
+            for (int i = 0; i < kSize / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+            return;
+        }
+        if constexpr (DT == AW4_F32) {
+            // the one aligned group of four words among the eight, the others by themselves
+            const int head = (int)((16 - ((uintptr_t)p & 15)) & 15) >> 2;
+            uint32_t v[7];
+#pragma unroll
+            for (int i = 0; i < 7; ++i) v[i] = w[i];
+            if (head & 2)
+#pragma unroll
+                for (int i = 0; i < 5; ++i) v[i] = v[i + 2];
+            if (head & 1)
+#pragma unroll
+                for (int i = 0; i < 6; ++i) v[i] = v[i + 1];
+            uint32_t* o = reinterpret_cast<uint32_t*>(p);
+            *reinterpret_cast<uint4*>(o + head) = make_uint4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < head || i >= head + 4) o[i] = w[i];
+        } else if ((uintptr_t)p & 2) {
+            uint16_t* o = reinterpret_cast<uint16_t*>(p);
+            o[0] = (uint16_t)w[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                *reinterpret_cast<uint32_t*>(o + 1 + 2 * i) = __funnelshift_r(w[i], w[i + 1], 16);
+            o[7] = (uint16_t)(w[3] >> 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+        }
+        return;
+    }
+    if constexpr (DT == AW4_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < cols) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < cols) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+    }
 }
 
 template <int DT>
@@ -108,55 +191,61 @@ __device__ __forceinline__ Raw8<DT> narrow8(const float v[8]) {
     return r;
 }
 
+// Larger magnitude of two words' values (its sign is not meaningful); a NaN is above every number.
 template <int DT>
-__device__ __forceinline__ void store_raw8(void* base, int64_t row_off, int col, int cols, bool vec,
-                                           const Raw8<DT>& r) {
-    if (vec && col + 8 <= cols) {
-        char* p = static_cast<char*>(base) + (row_off + col) * Elem<DT>::kBytes;
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == AW4_F32) asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (DT == AW4_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+struct A8Block {
+    int byte;       // e + 127, or kA8Nan
+    float most;     // largest magnitude
+};
+
+// The exponent of a block whose four lanes hold eight values each.
+template <int DT>
+__device__ __forceinline__ A8Block a8_block(const Raw8<DT>& r) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+    constexpr int kWords = Elem<DT>::kBytes * 2;
+    uint32_t m = larger<DT>(w[0], w[1]);
 #pragma unroll
-        for (int i = 0; i < Elem<DT>::kBytes / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+    for (int i = 2; i < kWords; ++i) m = larger<DT>(m, w[i]);
+    m = larger<DT>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = larger<DT>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if constexpr (DT == AW4_F32) {
+        m &= 0x7fffffffu;
     } else {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
-        if constexpr (DT == AW4_F32) {
-            uint32_t* p = static_cast<uint32_t*>(base) + row_off;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (col + i < cols) p[col + i] = w[i];
-        } else {
-            uint16_t* p = static_cast<uint16_t*>(base) + row_off;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (col + i < cols) p[col + i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
-        }
+        m &= 0x7fff7fffu;
+        m = max(m & 0xffffu, m >> 16);             // as integers, like the magnitudes
+        if constexpr (DT == AW4_BF16) m <<= 16;
+        else m = __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
     }
+    const int field = (int)(m >> 23);              // floor(log2) + 127; 255: not finite
+    return {field == 255 ? kA8Nan : max(field - 6, kA8MinByte<DT>), __uint_as_float(m)};
 }
 
-// Scale byte of a block whose four lanes hold eight values each.  The maximum
-// is taken over magnitude bits as integers, where a NaN is above every number.
-template <int DT>
-__device__ __forceinline__ int a8_scale_byte(const float v[8]) {
-    uint32_t m = 0;
+// The eight codes.  Adding 1.5 * 2^23 leaves rn(x * 2^-e), ties to even, in
+// the low bits of the sum.  Only a block whose largest magnitude is 127.5 steps or
+// more rounds to 128: the warp looks once whether it has one.
+__device__ __forceinline__ uint2 a8_encode8(const float v[8], const A8Block& b) {
+    const float inv = __uint_as_float(b.byte == kA8Nan ? 0u : (uint32_t)(254 - b.byte) << 23);
+    const f2 inv2 = pk2(inv, inv), magic = pk2(12582912.0f, 12582912.0f);
+    float t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const int field = (int)(m >> 23);                       // floor(log2) + 127; 255: not finite
-    return field == 255 ? kA8Nan : max(field - 6, kA8MinByte<DT>);
-}
-
-// The eight codes under scale byte b.  Adding 1.5 * 2^23 leaves rn(x * 2^-e),
-// ties to even, in the low bits of the sum.
-__device__ __forceinline__ uint2 a8_encode8(const float v[8], int b) {
-    const float inv = __uint_as_float(b == kA8Nan ? 0u : (uint32_t)(254 - b) << 23);
-    uint32_t t[8];
+    for (int i = 0; i < 8; i += 2) upk2(f2_fma(pk2(v[i], v[i + 1]), inv2, magic), t[i], t[i + 1]);
+    if (__any_sync(0xffffffffu, b.most * inv >= 127.5f))
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float s = __fmaf_rn(v[i], inv, 12582912.0f);
-        t[i] = __float_as_uint(fminf(fmaxf(s, 12582912.0f - 127.0f), 12582912.0f + 127.0f));
-    }
+        for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(t[i], 12582912.0f - 127.0f), 12582912.0f + 127.0f);
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(t[i]);
     uint2 r;
-    r.x = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
-    r.y = __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410);
+    r.x = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    r.y = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
     return r;
 }
 
@@ -164,18 +253,17 @@ __device__ __forceinline__ float a8_scale(int b) {
     return __uint_as_float(b == kA8Nan ? 0x7fc00000u : (uint32_t)b << 23);
 }
 
-// q * 2^e of four codes.  q + 128 in the low bits of 2^23 is the float
-// 2^23 + 128 + q; the subtraction and the product are both exact.
-__device__ __forceinline__ void a8_decode4(uint32_t w, float s, float v[4]) {
-    w ^= 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.0f) * s;
-}
-
+// q * 2^e of eight codes.  q + 128 in the low bits of 2^23 is the float
+// 2^23 + 128 + q; the subtraction (a product by one and a sum) and the product are exact.
 __device__ __forceinline__ void a8_decode8(uint2 w, float s, float v[8]) {
-    a8_decode4(w.x, s, v);
-    a8_decode4(w.y, s, v + 4);
+    const f2 one = pk2(1.0f, 1.0f), off = pk2(-8388736.0f, -8388736.0f), ss = pk2(s, s);
+    const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float a = __uint_as_float(__byte_perm(u[i / 4], 0x4b000000u, 0x7540 + i % 4));
+        const float b = __uint_as_float(__byte_perm(u[i / 4], 0x4b000000u, 0x7541 + i % 4));
+        upk2(f2_mul(f2_fma(pk2(a, b), one, off), ss), v[i], v[i + 1]);
+    }
 }
 
 // Where a lane's chunk of eight values lies: chunk `unit` of the

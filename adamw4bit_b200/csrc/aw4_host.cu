@@ -44,6 +44,16 @@ int32_t fail(int32_t code, const char* fmt, ...) {
 
 void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
+int sm_count(int device) {
+    static std::atomic<int> known[64];
+    if (device >= 0 && device < 64)
+        if (const int n = known[device].load(std::memory_order_relaxed)) return n;
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 1;
+    if (device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 static uint32_t fbits(float f) {
     uint32_t u;
     std::memcpy(&u, &f, 4);

@@ -14,6 +14,9 @@ int32_t fail(int32_t code, const char* fmt, ...);
 // Counts kernel launches (reported by aw4_launch_count()).
 void note_launch();
 
+// Multiprocessors of a device, asked for once.
+int sm_count(int device);
+
 // Makes `device` current for the duration of a call, restoring the caller's
 // device afterwards.
 class DeviceGuard {

@@ -47,13 +47,13 @@ constexpr uint32_t kKeyNegInf = 0x007fffffu;
 
 // A row belongs to L lanes; lane i holds experts [8 i, 8 i + 8) and, where V > 8, those 8 L further on.
 template <int DT, int L, int V>
-__device__ __forceinline__ void load_logits(const void* base, int64_t row, int64_t ld, int lane, int experts,
-                                            bool in, bool vec, float l[V]) {
+__device__ __forceinline__ void load_logits(const RowsIn& logits, int64_t row, int lane, int experts, bool in,
+                                            float l[V]) {
 #pragma unroll
     for (int c = 0; c < V / 8; ++c) {
         const int at = (c * L + lane) * 8;
         float v[8];
-        widen8<DT>(load_raw8<DT>(base, row * ld, at, in ? experts : 0, vec), v);
+        widen8<DT>(load_raw8<DT>(logits, in ? row : 0, at, in ? experts : 0), v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) l[c * 8 + i] = in && at + i < experts ? v[i] : -INFINITY;
     }
@@ -68,7 +68,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 template <int DT, int L, int V>
 __global__ void __launch_bounds__(kRouteThreads)
-route_forward_kernel(const void* __restrict__ logits, int64_t rows, int experts, int64_t ld, bool vec, int k,
+route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
                      const uint8_t* __restrict__ valid, bool renormalize, float* __restrict__ weights,
                      int32_t* __restrict__ chosen, float2* __restrict__ stats, float* __restrict__ psum,
                      int32_t* __restrict__ pcount) {
@@ -87,7 +87,7 @@ route_forward_kernel(const void* __restrict__ logits, int64_t rows, int experts,
         const bool in = row < rows;
         bool ok = in && (!valid || valid[row]);
         float l[V];
-        load_logits<DT, L, V>(logits, row, ld, lane, experts, ok, vec, l);
+        load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
         uint32_t key[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = order_key(l[i]);
@@ -193,11 +193,11 @@ route_finish_kernel(const float* __restrict__ psum, const int32_t* __restrict__ 
 
 template <int DT, int L, int V>
 __global__ void __launch_bounds__(kRouteThreads)
-route_backward_kernel(const void* __restrict__ logits, int64_t rows, int experts, int64_t ld, bool vec, int k,
+route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
                       bool renormalize, const float* __restrict__ weights, const int32_t* __restrict__ chosen,
                       const float2* __restrict__ stats, const int32_t* __restrict__ counts,
                       const float* __restrict__ dweights, const float* __restrict__ dbalance,
-                      void* __restrict__ dlogits, bool vec_out) {
+                      const RowsOut dlogits) {
     constexpr int kRows = kRouteThreads / L;
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
     const float n = fmaxf((float)counts[experts], 1.0f);
@@ -215,7 +215,7 @@ route_backward_kernel(const void* __restrict__ logits, int64_t rows, int experts
         const float2 st = in ? stats[row] : make_float2(0.0f, 0.0f);
         const bool ok = st.y != 0.0f;             // a NaN row is a valid one
         float l[V];
-        load_logits<DT, L, V>(logits, row, ld, lane, experts, ok, vec, l);
+        load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -240,8 +240,7 @@ route_backward_kernel(const void* __restrict__ logits, int64_t rows, int experts
         if (in)
 #pragma unroll
             for (int c = 0; c < V / 8; ++c)
-                store_raw8<DT>(dlogits, row * experts, (c * L + lane) * 8, experts, vec_out,
-                               narrow8<DT>(l + c * 8));
+                store_raw8<DT>(dlogits, row, (c * L + lane) * 8, experts, narrow8<DT>(l + c * 8));
     }
 }
 
@@ -278,12 +277,6 @@ static int32_t check_route(const char* what, int dtype, int64_t rows, int64_t ex
     return AW4_OK;
 }
 
-static int route_sms(int device) {
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 1;
-    return sms;
-}
-
 static int route_lanes(int experts) {
     int lanes = 1;
     while (lanes < 32 && lanes * 8 < experts) lanes *= 2;
@@ -292,11 +285,16 @@ static int route_lanes(int experts) {
 
 static int route_grid(int device, int64_t rows, int experts) {
     const int per = kRouteThreads / route_lanes(experts);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, (int64_t)route_sms(device) * 2));
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, (int64_t)sm_count(device) * 2));
 }
 
 static bool route_vec(const void* p, int64_t ld, int dtype) {
     return (uintptr_t)p % 16 == 0 && ld * (dtype == AW4_F32 ? 4 : 2) % 16 == 0;
+}
+
+static RowsIn route_rows(const void* p, int64_t rows, int experts, int64_t ld, int dtype) {
+    const char* base = static_cast<const char*>(p);
+    return {base, base + ((rows - 1) * ld + experts) * (dtype == AW4_F32 ? 4 : 2), ld, route_vec(p, ld, dtype)};
 }
 
 }  // namespace aw4
@@ -334,7 +332,7 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
         return route_shape(experts, [&](auto lanes, auto v) {
             route_forward_kernel<dt.value, lanes.value, v.value>
                 <<<grid, kRouteThreads, (2 * experts + 1) * 4, s>>>(
-                    logits, rows, experts, ld, route_vec(logits, ld, dtype), k, valid, renormalize != 0, weights,
+                    route_rows(logits, rows, experts, ld, dtype), rows, experts, k, valid, renormalize != 0, weights,
                     chosen, reinterpret_cast<float2*>(stats), psum, pcount);
             note_launch();
             const cudaError_t e = cudaGetLastError();
@@ -362,12 +360,12 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
     return route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
             const int per = kRouteThreads / lanes.value;
-            const int grid = (int)std::min<int64_t>((rows + per - 1) / per, (int64_t)route_sms(device) * 8);
+            const int grid = (int)std::min<int64_t>((rows + per - 1) / per, (int64_t)sm_count(device) * 8);
             route_backward_kernel<dt.value, lanes.value, v.value>
                 <<<grid, kRouteThreads, 0, (cudaStream_t)stream>>>(
-                    logits, rows, experts, ld, route_vec(logits, ld, dtype), k, renormalize != 0, weights, chosen,
-                    reinterpret_cast<const float2*>(stats), counts, dweights, dbalance, dlogits,
-                    route_vec(dlogits, experts, dtype));
+                    route_rows(logits, rows, experts, ld, dtype), rows, experts, k, renormalize != 0, weights, chosen,
+                    reinterpret_cast<const float2*>(stats), counts, dweights, dbalance,
+                    RowsOut{static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)});
             note_launch();
             const cudaError_t e = cudaGetLastError();
             return e == cudaSuccess ? AW4_OK

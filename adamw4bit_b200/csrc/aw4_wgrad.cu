@@ -606,8 +606,10 @@ weight_grad_join_kernel(const WgParams p, int pairs) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) *reinterpret_cast<float4*>(&tile[lane][(q * 8 + warp) * 4]) = acc[q];
     __syncthreads();
+    const RowsOut out = {static_cast<char*>(p.out), p.k, p.vec_out};
+    const RowsIn old = {out.base, out.base + (int64_t)p.groups * p.n * p.k * Elem<OT>::kBytes, p.k, p.vec_out};
     for (int r = warp; r < kWgSlice && t.n0 + row0 + r < p.n; r += 8) {
-        const int64_t row_off = ((int64_t)t.g * p.n + t.n0 + row0 + r) * p.k;
+        const int64_t row = (int64_t)t.g * p.n + t.n0 + row0 + r;
         const int at = t.k0 + lane * 8;
         if (at >= p.k) continue;
         float f[8];
@@ -615,11 +617,11 @@ weight_grad_join_kernel(const WgParams p, int pairs) {
         for (int i = 0; i < 8; ++i) f[i] = tile[r][lane * 8 + i];
         if (p.accumulate) {
             float o[8];
-            widen8<OT>(load_raw8<OT>(p.out, row_off, at, p.k, p.vec_out), o);
+            widen8<OT>(load_raw8<OT>(old, row, at, p.k), o);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] += o[i];
         }
-        store_raw8<OT>(p.out, row_off, at, p.k, p.vec_out, narrow8<OT>(f));
+        store_raw8<OT>(out, row, at, p.k, narrow8<OT>(f));
     }
 }
 
@@ -664,8 +666,7 @@ static int64_t wg_tiles(int64_t n, int64_t k) {
 constexpr int64_t kWgMinSteps = 4;
 
 static int wg_pairs(int device, int64_t rows, int64_t n, int64_t k, int64_t groups) {
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 2) sms = 2;
+    const int sms = std::max(2, sm_count(device));
     const int64_t tiles = wg_tiles(n, k);
     const int64_t steps = std::max<int64_t>(groups, (rows + kWgRows - 1) / kWgRows) * tiles;
     const int64_t want = std::max(tiles * groups, steps / kWgMinSteps);
