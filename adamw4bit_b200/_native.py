@@ -179,9 +179,12 @@ def require_cuda(t: torch.Tensor, what: str) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    if device.index is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return torch._C._cuda_getCurrentRawStream(device.index)   # the same handle without a Stream object
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The handle of a device's current stream by the device's number, without a Stream object (2 us).
+stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

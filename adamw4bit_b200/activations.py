@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import functools
 import math
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -44,33 +44,17 @@ __all__ = [
 BLOCK = 32
 
 
-def _nbytes(rows: int, cols: int) -> int:
-    """Bytes of a checkpoint: codes [rows][cols rounded up to 32], then a byte for each block."""
-    return rows * (-(-cols // BLOCK)) * (BLOCK + 1)
-
-
 class Act8:
     """The 8-bit checkpoint of a tensor: its codes and block exponents in one buffer (``data``), and the
     shape and dtype it reads back as.  ``codes`` is int8 [rows, cols rounded up to 32], ``scales`` uint8
     [rows, blocks] with e + 127 (255: the block was not finite)."""
 
-    __slots__ = ("data", "shape", "dtype")
+    __slots__ = ("data", "shape", "dtype", "rows", "cols")
 
     def __init__(self, data: torch.Tensor, shape, dtype: torch.dtype):
-        self.data, self.shape, self.dtype = data, torch.Size(shape), dtype
-
-    @classmethod
-    def empty(cls, shape, dtype: torch.dtype, device) -> "Act8":
-        rows, cols = math.prod(shape[:-1]), shape[-1]
-        return cls(torch.empty(_nbytes(rows, cols), dtype=torch.uint8, device=device), shape, dtype)
-
-    @property
-    def rows(self) -> int:
-        return math.prod(self.shape[:-1])
-
-    @property
-    def cols(self) -> int:
-        return self.shape[-1]
+        self.data, self.shape, self.dtype = data, shape, dtype
+        self.cols = shape[-1]
+        self.rows = math.prod(shape[:-1])
 
     @property
     def device(self) -> torch.device:
@@ -96,16 +80,25 @@ class Act8:
     def record_stream(self, stream) -> None:
         self.data.record_stream(stream)
 
-    def _ptrs(self) -> tuple[int, int]:
-        p = self.data.data_ptr()
-        return p, p + self.rows * (-(-self.cols // BLOCK)) * BLOCK
-
     def __repr__(self) -> str:
         return f"Act8(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
 
 
-@dataclass(frozen=True)
-class RMSNormSaved:
+def _empty_act8(t: torch.Tensor, shape, rows: int, cols: int) -> Act8:
+    """A checkpoint to be written for a tensor like t of this shape."""
+    x8 = Act8.__new__(Act8)
+    x8.data = t.new_empty(rows * (-(-cols // BLOCK)) * (BLOCK + 1), dtype=torch.uint8)
+    x8.shape, x8.dtype, x8.rows, x8.cols = shape, t.dtype, rows, cols
+    return x8
+
+
+def _ptrs(x8: Act8) -> tuple[int, int]:
+    """Addresses of codes and scales."""
+    p = x8.data.data_ptr()
+    return p, p + x8.rows * (-(-x8.cols // BLOCK)) * BLOCK
+
+
+class RMSNormSaved(NamedTuple):
     """What ``rms_norm_forward`` keeps: the checkpoint of x and (mean(x^2) + eps)^-1/2 of its rows.
     ``output`` is the checkpoint of y where it was asked for."""
     x8: Act8
@@ -113,8 +106,7 @@ class RMSNormSaved:
     output: Act8 | None = None
 
 
-@dataclass(frozen=True)
-class SwiGLUSaved:
+class SwiGLUSaved(NamedTuple):
     """What ``swiglu_forward`` keeps: the checkpoints of gate and up; ``packed`` where they came as halves
     of one tensor.  ``output`` is the checkpoint of h where it was asked for."""
     gate8: Act8
@@ -133,23 +125,24 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
 def _rows_of(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
     """t as rows of its last axis: (tensor, rows, cols, row stride).  A tensor whose leading axes have no
     single stride, or whose last axis is not contiguous, is copied."""
-    if t.dim() == 0:
+    if not t.is_cuda:
+        N.require_cuda(t, what)
+    shape = t.shape
+    if not shape:
         raise ValueError(f"{what}: a tensor of at least one dimension expected")
-    N.require_cuda(t, what)
+    cols = shape[-1]
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
     if t.is_contiguous():
-        cols = t.shape[-1]
-        return t, (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
-    cols = t.shape[-1]
-    rows = math.prod(t.shape[:-1])
+        return t, rows, cols, cols
     if cols <= 1 or t.stride(-1) == 1:
         ld, size = None, 1
-        for d in range(t.dim() - 2, -1, -1):
-            if t.shape[d] == 1:
+        for d in range(len(shape) - 2, -1, -1):
+            if shape[d] == 1:
                 continue
             if ld is None:
-                ld, size = t.stride(d), t.shape[d]
+                ld, size = t.stride(d), shape[d]
             elif t.stride(d) == ld * size:
-                size *= t.shape[d]
+                size *= shape[d]
             else:
                 break
         else:
@@ -158,8 +151,8 @@ def _rows_of(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
 
 
 def _same(a: torch.Tensor, device: torch.device, dtype: torch.dtype | None, what: str) -> None:
-    N.require_cuda(a, what)
     if a.device != device:
+        N.require_cuda(a, what)
         raise ValueError(f"{what}: on {a.device}, the others on {device}")
     if dtype is not None and a.dtype != dtype:
         raise TypeError(f"{what}: {dtype} expected, found {a.dtype}")
@@ -173,20 +166,21 @@ def quantize_act8(x: torch.Tensor) -> Act8:
     """The 8-bit checkpoint of x, blocks of 32 along its last axis."""
     code = _dtype_code(x, "quantize_act8")
     src, rows, cols, ld = _rows_of(x, "quantize_act8")
-    out = Act8.empty(x.shape, x.dtype, x.device)
-    codes, scales = out._ptrs()
-    N.check(N.lib().aw4_act8_quantize(src.data_ptr(), code, rows, cols, ld, codes, scales, x.device.index,
-                                      N.stream_handle(x.device)), "aw4_act8_quantize")
+    out = _empty_act8(x, x.shape, rows, cols)
+    codes, scales = _ptrs(out)
+    dev = x.get_device()
+    N.check(N.lib().aw4_act8_quantize(src.data_ptr(), code, rows, cols, ld, codes, scales, dev,
+                                      N.stream_of(dev)), "aw4_act8_quantize")
     return out
 
 
 def dequantize_act8(x8: Act8) -> torch.Tensor:
     """The values a checkpoint stands for, in its shape and dtype."""
-    out = torch.empty(x8.shape, dtype=x8.dtype, device=x8.device)
-    codes, scales = x8._ptrs()
+    out = x8.data.new_empty(x8.shape, dtype=x8.dtype)
+    codes, scales = _ptrs(x8)
+    dev = out.get_device()
     N.check(N.lib().aw4_act8_dequantize(codes, scales, N.DTYPE_CODES[x8.dtype], x8.rows, x8.cols,
-                                        out.data_ptr(), x8.cols, x8.device.index,
-                                        N.stream_handle(x8.device)), "aw4_act8_dequantize")
+                                        out.data_ptr(), x8.cols, dev, N.stream_of(dev)), "aw4_act8_dequantize")
     return out
 
 
@@ -216,16 +210,15 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *
     code = _dtype_code(x, "rms_norm")
     src, rows, cols, ld = _rows_of(x, "rms_norm")
     weight = _check_weight(weight, cols, x.dtype, x.device, "rms_norm")
-    dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-    x8 = Act8.empty(x.shape, x.dtype, dev)
-    y8 = Act8.empty(x.shape, x.dtype, dev) if checkpoint_output else None
-    yc, ys = y8._ptrs() if y8 is not None else (None, None)
+    dev = x.get_device()
+    y = x.new_empty(x.shape)
+    rstd = x.new_empty(rows, dtype=torch.float32)
+    x8 = _empty_act8(x, x.shape, rows, cols)
+    y8 = _empty_act8(x, x.shape, rows, cols) if checkpoint_output else None
+    yc, ys = _ptrs(y8) if y8 is not None else (None, None)
     N.check(N.lib().aw4_rms_norm_forward(src.data_ptr(), code, rows, cols, ld, weight.data_ptr(),
                                          N.DTYPE_CODES[weight.dtype], eps, y.data_ptr(), rstd.data_ptr(),
-                                         *x8._ptrs(), yc, ys, dev.index, N.stream_handle(dev)),
-            "aw4_rms_norm_forward")
+                                         *_ptrs(x8), yc, ys, dev, N.stream_of(dev)), "aw4_rms_norm_forward")
     return y, RMSNormSaved(x8, rstd, y8)
 
 
@@ -238,16 +231,15 @@ def rms_norm_backward(dy: torch.Tensor, weight: torch.Tensor,
         raise ValueError(f"rms_norm_backward: dy of shape {tuple(x8.shape)} expected, found {tuple(dy.shape)}")
     src, rows, cols, ld = _rows_of(dy, "rms_norm_backward")
     weight = _check_weight(weight, cols, x8.dtype, x8.device, "rms_norm_backward")
-    dev = dy.device
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    dw = torch.empty(cols, dtype=weight.dtype, device=dev)
-    nbytes = _norm_workspace(rows, cols, dev.index)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    N.check(N.lib().aw4_rms_norm_backward(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, cols, ld, *x8._ptrs(),
+    dev = dy.get_device()
+    dx = dy.new_empty(dy.shape)
+    dw = torch.empty_like(weight)
+    nbytes = _norm_workspace(rows, cols, dev)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    N.check(N.lib().aw4_rms_norm_backward(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, cols, ld, *_ptrs(x8),
                                           saved.rstd.data_ptr(), weight.data_ptr(),
                                           N.DTYPE_CODES[weight.dtype], dx.data_ptr(), dw.data_ptr(),
-                                          ws.data_ptr(), nbytes, dev.index, N.stream_handle(dev)),
-            "aw4_rms_norm_backward")
+                                          ws.data_ptr(), nbytes, dev, N.stream_of(dev)), "aw4_rms_norm_backward")
     return dx, dw
 
 
@@ -288,7 +280,6 @@ def swiglu_forward(gate: torch.Tensor, up: torch.Tensor | None = None, *,
     code = _dtype_code(gate, "swiglu")
     packed = up is None
     src, rows, cols, ld = _rows_of(gate, "swiglu")
-    dev = gate.device
     if packed:
         if cols % 2:
             raise ValueError(f"swiglu: gate and up as halves of the last axis expected, found {cols} columns")
@@ -296,19 +287,19 @@ def swiglu_forward(gate: torch.Tensor, up: torch.Tensor | None = None, *,
         shape = (*gate.shape[:-1], cols)
         other, ld_up = src.data_ptr() + cols * src.element_size(), ld
     else:
-        _same(up, dev, gate.dtype, "swiglu: up")
+        _same(up, gate.device, gate.dtype, "swiglu: up")
         if up.shape != gate.shape:
             raise ValueError(f"swiglu: up of shape {tuple(gate.shape)} expected, found {tuple(up.shape)}")
         shape = gate.shape
         up, _, _, ld_up = _rows_of(up, "swiglu")
         other = up.data_ptr()
-    h = torch.empty(shape, dtype=gate.dtype, device=dev)
-    g8, u8 = Act8.empty(shape, gate.dtype, dev), Act8.empty(shape, gate.dtype, dev)
-    h8 = Act8.empty(shape, gate.dtype, dev) if checkpoint_output else None
-    hc, hs = h8._ptrs() if h8 is not None else (None, None)
+    dev = gate.get_device()
+    h = gate.new_empty(shape)
+    g8, u8 = _empty_act8(gate, shape, rows, cols), _empty_act8(gate, shape, rows, cols)
+    h8 = _empty_act8(gate, shape, rows, cols) if checkpoint_output else None
+    hc, hs = _ptrs(h8) if h8 is not None else (None, None)
     N.check(N.lib().aw4_swiglu_forward(src.data_ptr(), other, code, rows, cols, ld, ld_up, h.data_ptr(),
-                                       *g8._ptrs(), *u8._ptrs(), hc, hs, dev.index, N.stream_handle(dev)),
-            "aw4_swiglu_forward")
+                                       *_ptrs(g8), *_ptrs(u8), hc, hs, dev, N.stream_of(dev)), "aw4_swiglu_forward")
     return h, SwiGLUSaved(g8, u8, packed, h8)
 
 
@@ -319,18 +310,18 @@ def swiglu_backward(dh: torch.Tensor, saved: SwiGLUSaved):
     if dh.shape != g8.shape:
         raise ValueError(f"swiglu_backward: dh of shape {tuple(g8.shape)} expected, found {tuple(dh.shape)}")
     src, rows, cols, ld = _rows_of(dh, "swiglu_backward")
-    dev = dh.device
+    dev = dh.get_device()
     if saved.packed:
-        both = torch.empty((*dh.shape[:-1], 2 * cols), dtype=dh.dtype, device=dev)
+        both = dh.new_empty((*dh.shape[:-1], 2 * cols))
         out, ld_out = both, 2 * cols
         dgate, dup = both.data_ptr(), both.data_ptr() + cols * both.element_size()
     else:
-        out = torch.empty(dh.shape, dtype=dh.dtype, device=dev), torch.empty(dh.shape, dtype=dh.dtype, device=dev)
+        out = dh.new_empty(dh.shape), dh.new_empty(dh.shape)
         ld_out = cols
         dgate, dup = out[0].data_ptr(), out[1].data_ptr()
-    N.check(N.lib().aw4_swiglu_backward(src.data_ptr(), N.DTYPE_CODES[dh.dtype], rows, cols, ld, *g8._ptrs(),
-                                        *saved.up8._ptrs(), dgate, dup, ld_out, dev.index,
-                                        N.stream_handle(dev)), "aw4_swiglu_backward")
+    N.check(N.lib().aw4_swiglu_backward(src.data_ptr(), N.DTYPE_CODES[dh.dtype], rows, cols, ld, *_ptrs(g8),
+                                        *_ptrs(saved.up8), dgate, dup, ld_out, dev, N.stream_of(dev)),
+            "aw4_swiglu_backward")
     return out
 
 
@@ -386,10 +377,10 @@ def weight_grad(dy: torch.Tensor, x8: Act8, offsets: torch.Tensor | None = None,
     if dy.dim() == 0 or dy.shape[:-1] != x8.shape[:-1]:
         raise ValueError(f"weight_grad: dy {tuple(dy.shape)} and the checkpoint {tuple(x8.shape)} differ in rows")
     src, rows, n, ld = _rows_of(dy, "weight_grad")
-    k, dev, groups = x8.cols, dy.device, 1
+    k, dev, groups = x8.cols, dy.get_device(), 1
     shape = (n, k)
     if offsets is not None:
-        _same(offsets, dev, torch.int32, "weight_grad: offsets")
+        _same(offsets, dy.device, torch.int32, "weight_grad: offsets")
         if offsets.dim() != 1 or offsets.numel() < 2:
             raise ValueError(f"weight_grad: offsets of groups + 1 values expected, found {tuple(offsets.shape)}")
         offsets = offsets.contiguous()
@@ -398,24 +389,23 @@ def weight_grad(dy: torch.Tensor, x8: Act8, offsets: torch.Tensor | None = None,
     if out is None:
         if accumulate:
             raise ValueError("weight_grad: accumulate needs out")
-        out = torch.empty(shape, dtype=out_dtype or dy.dtype, device=dev)
+        out = dy.new_empty(shape, dtype=out_dtype or dy.dtype)
     else:
-        _same(out, dev, out_dtype, "weight_grad: out")
+        _same(out, dy.device, out_dtype, "weight_grad: out")
         if out.shape != shape or not out.is_contiguous():
             raise ValueError(f"weight_grad: contiguous out of shape {shape} expected, found {tuple(out.shape)}")
     if out.dtype not in (dy.dtype, torch.float32):
         raise TypeError(f"weight_grad: result in {dy.dtype} or float32 expected, found {out.dtype}")
     if rows and (ld < n or ld % 8 or src.data_ptr() % 16):
         # the bulk copies want rows on 16 bytes
-        padded = torch.empty((rows, -(-n // 8) * 8), dtype=dy.dtype, device=dev)
+        padded = dy.new_empty((rows, -(-n // 8) * 8))
         padded[:, :n].copy_(src.reshape(rows, n))
         src, ld = padded, padded.shape[1]
-    nbytes = _wgrad_workspace(rows, n, k, groups, dev.index)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    N.check(N.lib().aw4_weight_grad(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, n, ld, *x8._ptrs(), k,
+    nbytes = _wgrad_workspace(rows, n, k, groups, dev)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    N.check(N.lib().aw4_weight_grad(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, n, ld, *_ptrs(x8), k,
                                     N.ptr(offsets), groups, out.data_ptr(), N.DTYPE_CODES[out.dtype],
-                                    int(accumulate), N.ptr(ws), nbytes, N.wait_status(), dev.index, N.stream_handle(dev)),
-            "aw4_weight_grad")
+                                    int(accumulate), N.ptr(ws), nbytes, N.wait_status(), dev, N.stream_of(dev)), "aw4_weight_grad")
     return out
 
 

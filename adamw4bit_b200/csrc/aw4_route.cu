@@ -29,34 +29,12 @@
 
 namespace aw4 {
 
-constexpr int kRouteThreads = 256;
 constexpr int kRouteMaxK = 32;
 
-// Logits as integers whose order is that of the numbers, -0 = +0, NaN on top.
-__device__ __forceinline__ uint32_t order_key(float l) {
-    uint32_t u = __float_as_uint(l);
-    if (l != l) return 0xffffffffu;
-    if (l == 0.0f) u = 0;
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-    if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
-    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-constexpr uint32_t kKeyNegInf = 0x007fffffu;
-
 // A row belongs to L lanes; lane i holds experts [8 i, 8 i + 8) and, where V > 8, those 8 L further on.
-template <int DT, int L, int V>
-__device__ __forceinline__ void load_logits(const RowsIn& logits, int64_t row, int lane, int experts, bool in,
-                                            float l[V]) {
-#pragma unroll
-    for (int c = 0; c < V / 8; ++c) {
-        const int at = (c * L + lane) * 8;
-        float v[8];
-        widen8<DT>(load_raw8<DT>(logits, in ? row : 0, at, in ? experts : 0), v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) l[c * 8 + i] = in && at + i < experts ? v[i] : -INFINITY;
-    }
+template <int L>
+__device__ __forceinline__ int expert_of(int lane, int i) {
+    return (i / 8 * L + lane) * 8 + i % 8;
 }
 
 template <int L>
@@ -65,22 +43,175 @@ __device__ __forceinline__ float lanes_sum(float v) {
     for (int o = L / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+__device__ __forceinline__ float exp_near(float x) {       // 2^-22 of the value, and 2^-24 |x| of it
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+    return r;
+}
+
+// The logits' order as unsigned integers: -0 = +0, NaN on top, 0 for a logit that takes no part.
+constexpr uint32_t kKeyNegInf = 0x007fffffu;
+
+__device__ __forceinline__ uint32_t order_key(float l) {
+    const uint32_t u = __float_as_uint(l + 0.0f);                     // -0 + 0 = +0
+    const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return l != l ? 0xffffffffu : k;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+struct Pick {
+    float value;
+    int expert;       // -1: none left above -inf
+};
+
+// Takes a row's logits from the largest down.  float32: the largest key left by a scan and
+// shuffles, then the lowest lane and place that has it by a ballot.
+template <int DT, int L, int V, bool kPacked = DT != AW4_F32>
+struct Picker {
+    uint32_t key[V];
+    __device__ __forceinline__ Picker(const float l[V], int lane, int experts, bool ok) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = ok && expert_of<L>(lane, i) < experts ? order_key(l[i]) : 0u;
+    }
+    __device__ __forceinline__ Pick next(int lane) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = max(best, key[i]);
+        best = lanes_max<L>(best);
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i)
+            if (key[i] == best) at = expert_of<L>(lane, i);
+        if constexpr (V == 8) {
+            // lanes hold ascending experts: the first lane that has it
+            const uint32_t here = (threadIdx.x & 31) & ~(L - 1);
+            const uint32_t has = __ballot_sync(0xffffffffu, at != 0x7fffffff) >> here;
+            at = __shfl_sync(0xffffffffu, at, here + (L == 32 ? __ffs(has) : __ffs(has & ((1u << (L & 31)) - 1))) - 1);
+        } else {
+#pragma unroll
+            for (int o = L / 2; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at == expert_of<L>(lane, i)) key[i] = 0;
+        return {key_value(best), best > kKeyNegInf ? at : -1};
+    }
+};
+
+// 16-bit logits: their order in the upper half of a word and the index, counted
+// down, in the lower.  Words are then all different and one maximum gives both.
+// Eight of a lane are sorted once; a lane's largest is then its first.
+template <int DT, int L, int V>
+struct Picker<DT, L, V, true> {
+    uint32_t key[V];
+    static constexpr uint32_t kNegInf = DT == AW4_BF16 ? 0x007fu : 0x03ffu;
+
+    __device__ __forceinline__ Picker(const float l[V], int lane, int experts, bool ok) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = expert_of<L>(lane, i);
+            const float z = l[i] + 0.0f;
+            const uint32_t u = DT == AW4_BF16 ? __float_as_uint(z)
+                                              : (uint32_t)__half_as_ushort(__float2half_rn(z)) << 16;
+            const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+            key[i] = !(ok && e < experts) ? 0u
+                     : l[i] != l[i]       ? 0xffff0000u | (0xffffu - e)
+                                          : (k & 0xffff0000u) | (0xffffu - e);
+        }
+        if constexpr (V == 8) {
+            constexpr int kA[19] = {0, 2, 4, 6, 0, 1, 4, 5, 1, 5, 0, 1, 2, 3, 2, 3, 1, 3, 5};
+            constexpr int kB[19] = {1, 3, 5, 7, 2, 3, 6, 7, 2, 6, 4, 5, 6, 7, 4, 5, 2, 4, 6};
+#pragma unroll
+            for (int c = 0; c < 19; ++c) {
+                const uint32_t a = key[kA[c]], b = key[kB[c]];
+                key[kA[c]] = max(a, b);
+                key[kB[c]] = min(a, b);
+            }
+        }
+    }
+    __device__ __forceinline__ Pick next(int) {
+        uint32_t mine = key[0];
+        if constexpr (V != 8)
+#pragma unroll
+            for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
+        const uint32_t best = lanes_max<L>(mine);
+        if constexpr (V == 8) {
+            const bool won = key[0] == best;
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = won ? (i + 1 < V ? key[i + 1] : 0u) : key[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (key[i] == best) key[i] = 0;
+        }
+        const uint32_t top = best >> 16;
+        float value;
+        if (top == 0xffffu) {
+            value = __uint_as_float(0x7fc00000u);
+        } else {
+            const uint32_t u = (top & 0x8000u) ? top & 0x7fffu : ~top & 0xffffu;
+            value = DT == AW4_BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+        }
+        return {value, top > kNegInf ? (int)(0xffffu - (best & 0xffffu)) : -1};
+    }
+};
 
 template <int DT, int L, int V>
-__global__ void __launch_bounds__(kRouteThreads)
-route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
-                     const uint8_t* __restrict__ valid, bool renormalize, float* __restrict__ weights,
-                     int32_t* __restrict__ chosen, float2* __restrict__ stats, float* __restrict__ psum,
-                     int32_t* __restrict__ pcount) {
-    constexpr int kRows = kRouteThreads / L;
+__device__ __forceinline__ void load_logits(const RowsIn& logits, int64_t row, int lane, int experts, bool in,
+                                            float l[V]) {
+#pragma unroll
+    for (int c = 0; c < V / 8; ++c)
+        widen8<DT>(load_raw8<DT>(logits, in ? row : 0, (c * L + lane) * 8, in ? experts : 0), l + c * 8);
+}
+
+// Threads of a forward block: a block an SM, its sums over rows in registers.
+template <int V>
+constexpr int kRouteThreads = V == 8 ? 1024 : V == 16 ? 512 : 256;
+
+// Balance loss from all experts' sums; called by a whole block.
+template <int T>
+__device__ __forceinline__ void finish_balance(float mine, int n, int experts, int k, float* scratch, float* balance) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float s = 0.0f;
+        for (int i = 0; i < T / 32; ++i) s += scratch[i];
+        *balance = n ? s * ((float)experts / (float)k) / (float)n / (float)n : 0.0f;
+    }
+}
+
+template <int DT, int L, int V>
+__global__ void __launch_bounds__(kRouteThreads<V>, 1)
+route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, const uint8_t* __restrict__ valid,
+                     bool renormalize, float* __restrict__ weights, int32_t* __restrict__ chosen,
+                     float2* __restrict__ stats, float* __restrict__ psum, int32_t* __restrict__ pcount,
+                     int32_t* __restrict__ counts, float* __restrict__ balance) {
+    constexpr int kThreads = kRouteThreads<V>, kRows = kThreads / L;
     extern __shared__ int32_t smem[];
-    int32_t* count = smem;                                        // [experts + 1], the last: valid rows
-    float* sums = reinterpret_cast<float*>(smem + experts + 1);   // [experts]
-    for (int i = threadIdx.x; i <= experts; i += kRouteThreads) count[i] = 0;
-    for (int i = threadIdx.x; i < experts; i += kRouteThreads) sums[i] = 0.0f;
+    int32_t* count = smem;                                            // [experts + 1], the last: valid rows
+    float* sums = reinterpret_cast<float*>(count + experts + 1);      // [experts]
+    float* weight_s = sums + experts;                                 // [rows][k]
+    int32_t* chosen_s = reinterpret_cast<int32_t*>(weight_s + kRows * k);
+    for (int i = threadIdx.x; i <= experts; i += kThreads) count[i] = 0;
     __syncthreads();
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
-    float acc[V] = {};
+    float* my_weight = weight_s + group * k;
+    int32_t* my_chosen = chosen_s + group * k;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
     const int64_t tiles = (rows + kRows - 1) / kRows;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int64_t row = tile * kRows + group;
@@ -88,124 +219,135 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
         bool ok = in && (!valid || valid[row]);
         float l[V];
         load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
-        uint32_t key[V];
+        Picker<DT, L, V> picker(l, lane, experts, ok);
+        Pick pick = picker.next(lane);
+        ok = ok && pick.expert >= 0;
+        const float top = pick.value;
+        float part = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = order_key(l[i]);
-        float top = 0.0f, total = 0.0f, denominator = 0.0f;
-        for (int j = 0; j < k; ++j) {
-            // the largest key left, and the lowest index that has it
-            uint32_t best = 0;
-#pragma unroll
-            for (int i = 0; i < V; ++i) best = max(best, key[i]);
-#pragma unroll
-            for (int o = L / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-            int at = 0x7fffffff;
-#pragma unroll
-            for (int i = V - 1; i >= 0; --i)
-                if (key[i] == best) at = (i / 8 * L + lane) * 8 + i % 8;
-#pragma unroll
-            for (int o = L / 2; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (at == (i / 8 * L + lane) * 8 + i % 8) key[i] = 0;
-            const bool some = best > kKeyNegInf;
-            if (j == 0) {
-                ok = ok && some;
-                top = key_value(best);
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    l[i] = ok ? expf(l[i] - top) : 0.0f;
-                    part += l[i];
-                }
-                total = lanes_sum<L>(part);
-            }
-            const bool take = ok && some;
-            const float w = take ? expf(key_value(best) - top) : 0.0f;
-            denominator += w;
-            if (in && lane == 0) {
-                weights[row * k + j] = w;
-                chosen[row * k + j] = take ? at : -1;
-                if (take) atomicAdd(&count[at], 1);
-            }
+        for (int i = 0; i < V; ++i) {
+            l[i] = ok && expert_of<L>(lane, i) < experts ? exp_near(l[i] - top) : 0.0f;
+            part += l[i];
         }
+        const float total = lanes_sum<L>(part);
         const float inv = ok ? 1.0f / total : 0.0f;
-        if (in && lane == 0) {
-            stats[row] = make_float2(top, inv);
-            if (ok) atomicAdd(&count[experts], 1);
-            const float scale = !ok ? 0.0f : renormalize ? 1.0f / denominator : inv;
-            for (int j = 0; j < k; ++j) weights[row * k + j] *= scale;
-        }
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (ok) acc[i] = __fmaf_rn(l[i], inv, acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = ok ? __fmaf_rn(l[i], inv, acc[i]) : acc[i];
+        // the choices, by the lanes in turn; all lanes know each
+        float chosen_sum = 0.0f;
+        for (int j = 0; j < k; ++j) {
+            const bool take = ok && pick.expert >= 0;
+            const float w = take ? exp_near(pick.value - top) : 0.0f;
+            chosen_sum += w;
+            if (lane == j % L) {
+                my_weight[j] = w;
+                my_chosen[j] = take ? pick.expert : -1;
+                if (take) atomicAdd(&count[pick.expert], 1);
+            }
+            if (j + 1 < k) pick = picker.next(lane);
+        }
+        const float scale = !ok ? 0.0f : renormalize ? 1.0f / chosen_sum : inv;
+        if (in) {
+            if (lane == 0) {
+                stats[row] = make_float2(top, inv);
+                if (ok) atomicAdd(&count[experts], 1);
+            }
+            for (int j = lane; j < k; j += L) {       // its own choices
+                weights[row * k + j] = my_weight[j] * scale;
+                chosen[row * k + j] = my_chosen[j];
+            }
+        }
     }
     // groups of the warp, then the warps in turn
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int o = 16; o >= L; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    for (int w = 0; w < kRouteThreads / 32; ++w) {
-        __syncthreads();
-        if ((int)(threadIdx.x >> 5) == w && (threadIdx.x & 31) < L)
+    __syncthreads();
+    float* warp_sums = weight_s;                      // [kThreads / 32][V L]: the choices are out
+    if ((threadIdx.x & 31) < L)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int e = (i / 8 * L + lane) * 8 + i % 8;
-                if (e < experts) sums[e] += acc[i];
-            }
+        for (int i = 0; i < V; ++i) warp_sums[(threadIdx.x >> 5) * (V * L) + expert_of<L>(lane, i)] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        float s = 0.0f;
+#pragma unroll 8
+        for (int w = 0; w < kThreads / 32; ++w) s += warp_sums[w * (V * L) + e];
+        sums[e] = s;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < experts; i += kRouteThreads) psum[(int64_t)blockIdx.x * experts + i] = sums[i];
-    for (int i = threadIdx.x; i <= experts; i += kRouteThreads)
+    if (gridDim.x == 1) {
+        float mine = 0.0f;
+        for (int e = threadIdx.x; e <= experts; e += kThreads) {
+            counts[e] = count[e];
+            if (e < experts) mine = __fmaf_rn((float)count[e], sums[e], mine);
+        }
+        finish_balance<kThreads>(mine, count[experts], experts, k, warp_sums, balance);
+        return;
+    }
+    for (int i = threadIdx.x; i < experts; i += kThreads) psum[(int64_t)blockIdx.x * experts + i] = sums[i];
+    for (int i = threadIdx.x; i <= experts; i += kThreads)
         pcount[(int64_t)blockIdx.x * (experts + 1) + i] = count[i];
 }
 
-// One block: counts, the number of valid rows and the balance loss.
+// One block: counts, the number of valid rows and the balance loss from the blocks' parts.  1024 / C threads
+// share an expert's parts, C the experts rounded up to a power of two.
 __global__ void __launch_bounds__(1024)
 route_finish_kernel(const float* __restrict__ psum, const int32_t* __restrict__ pcount, int parts, int experts,
-                    int k, int32_t* __restrict__ counts, float* __restrict__ balance) {
-    __shared__ float warp_part[32];
-    __shared__ int valid_rows;
-    float mine = 0.0f;
-    for (int e = threadIdx.x; e <= experts; e += 1024) {
-        int c = 0;
-        for (int p = 0; p < parts; ++p) c += pcount[(int64_t)p * (experts + 1) + e];
-        counts[e] = c;
-        if (e == experts) {
-            valid_rows = c;
-        } else {
-            float s = 0.0f;
-            for (int p = 0; p < parts; ++p) s += psum[(int64_t)p * experts + e];
-            mine = __fmaf_rn((float)c, s, mine);
+                    int log_c, int k, int32_t* __restrict__ counts, float* __restrict__ balance) {
+    __shared__ float sum_s[1024], scratch[32];
+    __shared__ int count_s[1024], valid_rows;
+    const int c = 1 << log_c, e = threadIdx.x & (c - 1), slice = threadIdx.x >> log_c, slices = 1024 >> log_c;
+    if (threadIdx.x == 0) valid_rows = 0;
+    float s = 0.0f;
+    int n = 0;
+    if (e < experts)
+#pragma unroll 8
+        for (int p = slice; p < parts; p += slices) {
+            s += psum[(int64_t)p * experts + e];
+            n += pcount[(int64_t)p * (experts + 1) + e];
         }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = mine;
+    sum_s[threadIdx.x] = s;
+    count_s[threadIdx.x] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float s = 0.0f;
-        for (int i = 0; i < 32; ++i) s += warp_part[i];
-        const float n = (float)valid_rows;
-        *balance = valid_rows ? s * ((float)experts / (float)k) / n / n : 0.0f;
+    for (int p = threadIdx.x; p < parts; p += 1024) atomicAdd(&valid_rows, pcount[(int64_t)p * (experts + 1) + experts]);
+    float mine = 0.0f;
+    if (slice == 0 && e < experts) {
+        for (int i = 1; i < slices; ++i) {
+            s += sum_s[(i << log_c) + e];
+            n += count_s[(i << log_c) + e];
+        }
+        counts[e] = n;
+        mine = (float)n * s;
     }
+    __syncthreads();
+    if (threadIdx.x == 0) counts[experts] = valid_rows;
+    finish_balance<1024>(mine, valid_rows, experts, k, scratch, balance);
 }
 
+constexpr int kRouteBackThreads = 256;
+
 template <int DT, int L, int V>
-__global__ void __launch_bounds__(kRouteThreads)
-route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
-                      bool renormalize, const float* __restrict__ weights, const int32_t* __restrict__ chosen,
+__global__ void __launch_bounds__(kRouteBackThreads)
+route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, bool renormalize,
+                      const float* __restrict__ weights, const int32_t* __restrict__ chosen,
                       const float2* __restrict__ stats, const int32_t* __restrict__ counts,
                       const float* __restrict__ dweights, const float* __restrict__ dbalance,
                       const RowsOut dlogits) {
-    constexpr int kRows = kRouteThreads / L;
+    constexpr int kRows = kRouteBackThreads / L;
+    // t_j at its expert's place, zero elsewhere: written and cleared by the lanes that have the choices
+    __shared__ __align__(16) float place[kRows][V * L];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    float* mine = place[group];
+#pragma unroll
+    for (int i = 0; i < V; ++i) mine[expert_of<L>(lane, i)] = 0.0f;
+    __syncwarp();
     const float n = fmaxf((float)counts[experts], 1.0f);
     const float unit = dbalance ? *dbalance * ((float)experts / (float)k) / n / n : 0.0f;
     float share[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int e = (i / 8 * L + lane) * 8 + i % 8;
+        const int e = expert_of<L>(lane, i);
         share[i] = e < experts ? (float)counts[e] * unit : 0.0f;
     }
     const int64_t tiles = (rows + kRows - 1) / kRows;
@@ -216,31 +358,40 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k,
         const bool ok = st.y != 0.0f;             // a NaN row is a valid one
         float l[V];
         load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
+        const bool picks = dweights && ok;
+        float inner = 0.0f;
+        if (picks)
+            for (int j = lane; j < k; j += L)
+                if (chosen[row * k + j] >= 0)
+                    inner = __fmaf_rn(weights[row * k + j], dweights[row * k + j], inner);
+        inner = lanes_sum<L>(inner);
+        if (picks)
+            for (int j = lane; j < k; j += L) {
+                const int at = chosen[row * k + j];
+                if (at >= 0) mine[at] = weights[row * k + j] * (dweights[row * k + j] - (renormalize ? inner : 0.0f));
+            }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = ok ? expf(l[i] - st.x) * st.y : 0.0f;
+            l[i] = ok && expert_of<L>(lane, i) < experts ? exp_near(l[i] - st.x) * st.y : 0.0f;
             sum = __fmaf_rn(l[i], share[i], sum);
         }
         sum = lanes_sum<L>(sum);
-        float inner = 0.0f;
-        if (dweights && ok)
-            for (int j = 0; j < k; ++j) inner = __fmaf_rn(weights[row * k + j], dweights[row * k + j], inner);
-        const float off = renormalize ? sum : sum + inner, back = renormalize ? inner : 0.0f;
+        const float off = renormalize ? sum : sum + inner;
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < V; ++i) l[i] *= share[i] - off;
-        if (dweights && ok)
-            for (int j = 0; j < k; ++j) {
+        for (int i = 0; i < V; ++i) l[i] = __fmaf_rn(l[i], share[i] - off, mine[expert_of<L>(lane, i)]);
+        __syncwarp();
+        if (picks)
+            for (int j = lane; j < k; j += L) {
                 const int at = chosen[row * k + j];
-                const float t = weights[row * k + j] * (dweights[row * k + j] - back);
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (at == (i / 8 * L + lane) * 8 + i % 8) l[i] += t;
+                if (at >= 0) mine[at] = 0.0f;
             }
         if (in)
 #pragma unroll
             for (int c = 0; c < V / 8; ++c)
                 store_raw8<DT>(dlogits, row, (c * L + lane) * 8, experts, narrow8<DT>(l + c * 8));
+        __syncwarp();
     }
 }
 
@@ -283,9 +434,11 @@ static int route_lanes(int experts) {
     return lanes;
 }
 
+// Blocks of the forward kernel and threads of each: one an SM, or as many as have a row.
+static int route_threads(int experts) { return experts <= 256 ? 1024 : experts <= 512 ? 512 : 256; }
 static int route_grid(int device, int64_t rows, int experts) {
-    const int per = kRouteThreads / route_lanes(experts);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, (int64_t)sm_count(device) * 2));
+    const int per = route_threads(experts) / route_lanes(experts);
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, sm_count(device)));
 }
 
 static bool route_vec(const void* p, int64_t ld, int dtype) {
@@ -330,18 +483,28 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
     int32_t* pcount = reinterpret_cast<int32_t*>(psum + (int64_t)grid * experts);
     const int32_t rc = route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
-            route_forward_kernel<dt.value, lanes.value, v.value>
-                <<<grid, kRouteThreads, (2 * experts + 1) * 4, s>>>(
+            constexpr int kThreads = kRouteThreads<v.value>;
+            // choices of the rows in work, later the warps' sums
+            const int choices = std::max(2 * (kThreads / lanes.value) * k, kThreads / 32 * v.value * lanes.value);
+            auto kernel = route_forward_kernel<dt.value, lanes.value, v.value>;
+            const int bytes = (2 * experts + 1 + choices) * 4;
+            if (bytes > 48 * 1024) {
+                const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+                if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
+            }
+            kernel<<<grid, kThreads, bytes, s>>>(
                     route_rows(logits, rows, experts, ld, dtype), rows, experts, k, valid, renormalize != 0, weights,
-                    chosen, reinterpret_cast<float2*>(stats), psum, pcount);
+                    chosen, reinterpret_cast<float2*>(stats), psum, pcount, counts, balance);
             note_launch();
             const cudaError_t e = cudaGetLastError();
-            return e == cudaSuccess ? AW4_OK
+            return e == cudaSuccess ? (int32_t)AW4_OK
                                     : fail(AW4_ERR_CUDA, "route_forward launch: %s", cudaGetErrorString(e));
         });
     });
-    if (rc) return rc;
-    route_finish_kernel<<<1, 1024, 0, s>>>(psum, pcount, grid, experts, k, counts, balance);
+    if (rc || grid == 1) return rc;
+    int log_c = 0;
+    while ((1 << log_c) < experts) ++log_c;
+    route_finish_kernel<<<1, 1024, 0, s>>>(psum, pcount, grid, experts, log_c, k, counts, balance);
     note_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? AW4_OK : fail(AW4_ERR_CUDA, "route_finish launch: %s", cudaGetErrorString(e));
@@ -359,10 +522,10 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     return route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
-            const int per = kRouteThreads / lanes.value;
+            const int per = kRouteBackThreads / lanes.value;
             const int grid = (int)std::min<int64_t>((rows + per - 1) / per, (int64_t)sm_count(device) * 8);
             route_backward_kernel<dt.value, lanes.value, v.value>
-                <<<grid, kRouteThreads, 0, (cudaStream_t)stream>>>(
+                <<<grid, kRouteBackThreads, 0, (cudaStream_t)stream>>>(
                     route_rows(logits, rows, experts, ld, dtype), rows, experts, k, renormalize != 0, weights, chosen,
                     reinterpret_cast<const float2*>(stats), counts, dweights, dbalance,
                     RowsOut{static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)});

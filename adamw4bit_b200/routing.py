@@ -18,7 +18,6 @@ gives the offsets of ``activations.grouped_linear`` by a running sum (``group_of
 from __future__ import annotations
 
 import functools
-from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -40,8 +39,7 @@ class Routed(NamedTuple):
     balance_loss: torch.Tensor
 
 
-@dataclass(frozen=True)
-class Routing:
+class Routing(NamedTuple):
     """The outputs of ``route_forward`` and what its backward call reads: the logits as they were, each
     token's largest logit and 1 / sum exp, and the counts with the number of valid tokens behind them."""
     weights: torch.Tensor
@@ -70,23 +68,23 @@ def route_forward(logits: torch.Tensor, k: int, valid: torch.Tensor | None = Non
         raise ValueError(f"route: 1 to {MAX_EXPERTS} experts expected, found {experts}")
     if not 1 <= k <= min(experts, MAX_K):
         raise ValueError(f"route: k from 1 to {min(experts, MAX_K)} expected, found {k}")
-    dev, lead = logits.device, logits.shape[:-1]
+    dev, lead = logits.get_device(), logits.shape[:-1]
     if valid is not None:
-        _same(valid, dev, torch.bool, "route: valid")
+        _same(valid, logits.device, torch.bool, "route: valid")
         if valid.shape != lead:
             raise ValueError(f"route: valid of shape {tuple(lead)} expected, found {tuple(valid.shape)}")
         valid = valid.contiguous()
-    weights = torch.empty((*lead, k), dtype=torch.float32, device=dev)
-    chosen = torch.empty((*lead, k), dtype=torch.int32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    totals = torch.empty(experts + 1, dtype=torch.int32, device=dev)
-    balance = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = _workspace(rows, experts, dev.index)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    weights = logits.new_empty((*lead, k), dtype=torch.float32)
+    chosen = logits.new_empty((*lead, k), dtype=torch.int32)
+    stats = weights.new_empty((rows, 2))
+    totals = chosen.new_empty(experts + 1)
+    balance = weights.new_empty(())
+    nbytes = _workspace(rows, experts, dev)
+    ws = logits.new_empty(nbytes, dtype=torch.uint8)
     N.check(N.lib().aw4_route_forward(src.data_ptr(), code, rows, experts, ld, k, N.ptr(valid), int(renormalize),
                                       weights.data_ptr(), chosen.data_ptr(), stats.data_ptr(), totals.data_ptr(),
-                                      balance.data_ptr(), ws.data_ptr(), nbytes, dev.index,
-                                      N.stream_handle(dev)), "aw4_route_forward")
+                                      balance.data_ptr(), ws.data_ptr(), nbytes, dev, N.stream_of(dev)),
+            "aw4_route_forward")
     return Routing(weights, chosen, totals[:experts], balance, logits, stats, totals, k, renormalize)
 
 
@@ -97,6 +95,7 @@ def route_backward(dweights: torch.Tensor | None, dbalance: torch.Tensor | None,
     logits = routing.logits
     src, rows, experts, ld = _rows_of(logits, "route_backward")
     dev = logits.device
+    index = logits.get_device()
     if dweights is not None:
         _same(dweights, dev, torch.float32, "route_backward: dweights")
         if dweights.shape != routing.weights.shape:
@@ -107,13 +106,12 @@ def route_backward(dweights: torch.Tensor | None, dbalance: torch.Tensor | None,
         _same(dbalance, dev, torch.float32, "route_backward: dbalance")
         if dbalance.numel() != 1:
             raise ValueError(f"route_backward: a scalar dbalance expected, found {tuple(dbalance.shape)}")
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    dlogits = logits.new_empty(logits.shape)
     N.check(N.lib().aw4_route_backward(src.data_ptr(), N.DTYPE_CODES[logits.dtype], rows, experts, ld, routing.k,
                                        int(routing.renormalize), routing.weights.data_ptr(),
                                        routing.experts.data_ptr(), routing.stats.data_ptr(),
                                        routing.totals.data_ptr(), N.ptr(dweights), N.ptr(dbalance),
-                                       dlogits.data_ptr(), dev.index, N.stream_handle(dev)),
-            "aw4_route_backward")
+                                       dlogits.data_ptr(), index, N.stream_of(index)), "aw4_route_backward")
     return dlogits
 
 

@@ -224,3 +224,14 @@ def test_refusals():
         Q.route_backward(torch.zeros(4, 2, device=DEV).half(), None, r)
     with pytest.raises(ValueError):
         Q.route_backward(None, torch.zeros(2, device=DEV), r)
+
+
+def test_gradient_of_a_missing_choice_is_ignored():
+    logits = _logits(5, 8, torch.float32)
+    logits[2, 1:] = -math.inf                             # one expert for three choices
+    dw = torch.ones(5, 3)
+    dw[2, 1:] = math.nan
+    for renormalize in (True, False):
+        r = Q.route_forward(logits.to(DEV), 3, renormalize=renormalize)
+        dl = Q.route_backward(dw.to(DEV), None, r)
+        assert r.experts[2].tolist() == [0, -1, -1] and torch.isfinite(dl).all()
