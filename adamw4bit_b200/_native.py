@@ -112,8 +112,8 @@ SIGNATURES = {
     "aw4_weight_grad": ([_VP, _I32, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _VP, _I32, _I32, _VP, _I64,
                          _VP, _I32, _VP], _I32),
     "aw4_route_forward_workspace": ([_I64, _I32, _I32], _U64),
-    "aw4_route_forward": ([_VP, _I32, _I64, _I32, _I64, _I32, _VP, _I32, *[_VP] * 6, _I64, _I32, _VP], _I32),
-    "aw4_route_backward": ([_VP, _I32, _I64, _I32, _I64, _I32, _I32, *[_VP] * 7, _I32, _VP], _I32),
+    "aw4_route_forward": ([_VP, _I32, _I64, _I32, _I64, _I32, _VP, _I32, *[_VP] * 7, _I64, _I32, _VP], _I32),
+    "aw4_route_backward": ([_VP, _I32, _I64, _I32, _I64, _I32, _I32, *[_VP] * 8, _I32, _VP], _I32),
 }
 
 

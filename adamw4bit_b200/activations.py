@@ -234,9 +234,10 @@ def rms_norm_backward(dy: torch.Tensor, weight: torch.Tensor,
     dev = dy.get_device()
     dx = dy.new_empty(dy.shape)
     dw = torch.empty_like(weight)
+    code = N.DTYPE_CODES[dy.dtype]
     nbytes = _norm_workspace(rows, cols, dev)
     ws = dy.new_empty(nbytes, dtype=torch.uint8)
-    N.check(N.lib().aw4_rms_norm_backward(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, cols, ld, *_ptrs(x8),
+    N.check(N.lib().aw4_rms_norm_backward(src.data_ptr(), code, rows, cols, ld, *_ptrs(x8),
                                           saved.rstd.data_ptr(), weight.data_ptr(),
                                           N.DTYPE_CODES[weight.dtype], dx.data_ptr(), dw.data_ptr(),
                                           ws.data_ptr(), nbytes, dev, N.stream_of(dev)), "aw4_rms_norm_backward")

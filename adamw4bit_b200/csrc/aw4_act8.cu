@@ -109,7 +109,9 @@ __device__ __forceinline__ float sigmoid(float g) {
     }
 }
 
-constexpr int kGluChunks = 2, kGluRun = 32 * kGluChunks;
+// Chunks in flight: two forward (152 us at 8192 x 14336 bf16; 164 with one, 157 with four), one backward (149 us;
+// 167 with two, 205 with four).
+constexpr int kGluForward = 2, kGluBackward = 1;
 
 template <int DT, bool EMIT>
 __global__ void __launch_bounds__(kA8Threads)
@@ -118,19 +120,19 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
                       uint8_t* __restrict__ ucodes, uint8_t* __restrict__ uscales,
                       uint8_t* __restrict__ hcodes, uint8_t* __restrict__ hscales) {
     const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row, unit0 = warp_run(kGluRun);
+    const int64_t units = rows * per_row, unit0 = warp_run(32 * kGluForward);
     if (unit0 >= units) return;
     const RunAt run = run_at(unit0, per_row);
-    Raw8<DT> rg[kGluChunks], ru[kGluChunks];
-    ChunkAt at[kGluChunks];
+    Raw8<DT> rg[kGluForward], ru[kGluForward];
+    ChunkAt at[kGluForward];
 #pragma unroll
-    for (int j = 0; j < kGluChunks; ++j) {
+    for (int j = 0; j < kGluForward; ++j) {
         at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
         rg[j] = load_raw8<DT>(gate, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
         ru[j] = load_raw8<DT>(up, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
     }
 #pragma unroll
-    for (int j = 0; j < kGluChunks; ++j) {
+    for (int j = 0; j < kGluForward; ++j) {
         const int64_t u = unit0 + j * 32 + lane;
         float g[8], p[8], y[8];
         widen8<DT>(rg[j], g);
@@ -170,15 +172,15 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
                        const uint8_t* __restrict__ ucodes, const uint8_t* __restrict__ uscales,
                        const RowsOut dgate, const RowsOut dup) {
     const int lane = threadIdx.x & 31;
-    const int64_t units = rows * per_row, unit0 = warp_run(kGluRun);
+    const int64_t units = rows * per_row, unit0 = warp_run(32 * kGluBackward);
     if (unit0 >= units) return;
     const RunAt run = run_at(unit0, per_row);
-    Raw8<DT> rd[kGluChunks];
-    uint2 qg[kGluChunks], qu[kGluChunks];
-    int bg[kGluChunks], bu[kGluChunks];
-    ChunkAt at[kGluChunks];
+    Raw8<DT> rd[kGluBackward];
+    uint2 qg[kGluBackward], qu[kGluBackward];
+    int bg[kGluBackward], bu[kGluBackward];
+    ChunkAt at[kGluBackward];
 #pragma unroll
-    for (int j = 0; j < kGluChunks; ++j) {
+    for (int j = 0; j < kGluBackward; ++j) {
         const int64_t u = unit0 + j * 32 + lane;
         at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
         if (!at[j].in) continue;
@@ -189,7 +191,7 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
         bu[j] = uscales[u >> 2];
     }
 #pragma unroll
-    for (int j = 0; j < kGluChunks; ++j) {
+    for (int j = 0; j < kGluBackward; ++j) {
         if (!at[j].in) continue;
         float d[8], g[8], p[8], s[8], f[8];
         widen8<DT>(rd[j], d);
@@ -217,8 +219,10 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
 //
 // A row belongs to NT threads that hold V chunks of eight values each; NT = 32:
 // a warp a row, no barrier.  Blocks stay and walk the rows, the next row's loads on
-// their way while one is worked on: the weight is read once a block, and the
+// their way while one is worked on.  The weight waits in shared memory, and the
 // backward kernel keeps its columns' sum of dy v r in registers over all its rows.
+// Two chunks a thread: a row's own cost, the sum over its threads, is then half of
+// what one chunk a thread pays (forward 73 us at 16384 x 4096 bf16 with one).
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -243,38 +247,77 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[NT / 32], int sl
     }
 }
 
-__device__ __forceinline__ void load_weight8(const void* w, int dtype, int col, int cols, float v[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0.0f;
-        if (col + i < cols)
-            v[i] = dtype == AW4_F32    ? Elem<AW4_F32>::load1(w, col + i)
-                   : dtype == AW4_BF16 ? Elem<AW4_BF16>::load1(w, col + i)
-                                       : Elem<AW4_F16>::load1(w, col + i);
-    }
+// 1 / sqrt(x): the hardware's estimate and one step of Newton's method.
+__device__ __forceinline__ float inv_sqrt(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    const float e = __fmaf_rn(-x * r, r, 1.0f);
+    return x < INFINITY ? __fmaf_rn(0.5f * r, e, r) : r;       // infinity: 0, NaN: NaN
 }
 
+// A thread's chunks of the weight as float32 in shared memory, zeros behind the
+// last column: the first halves of all chunks, then the second, so that a warp
+// reads whole lines.  A thread reads what it wrote: no barrier.
 template <int NT, int V>
-constexpr int kNormBlocks = V > 1 ? 1 : NT == 32 ? 4 : 1024 / NT;      // resident on an SM
+__device__ __forceinline__ void stage_weight(const void* w, int dtype, int cols, int t, float4* s) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int u = j * NT + t, col = u * 8;
+        float v[8];
+        const char* p = static_cast<const char*>(w) + (int64_t)col * (dtype == AW4_F32 ? 4 : 2);
+        if (col + 8 <= cols && (uintptr_t)p % 16 == 0) {
+            if (dtype == AW4_F32) Elem<AW4_F32>::load8(w, col, v);
+            else if (dtype == AW4_BF16) Elem<AW4_BF16>::load8(w, col, v);
+            else Elem<AW4_F16>::load8(w, col, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = 0.0f;
+                if (col + i < cols)
+                    v[i] = dtype == AW4_F32    ? Elem<AW4_F32>::load1(w, col + i)
+                           : dtype == AW4_BF16 ? Elem<AW4_BF16>::load1(w, col + i)
+                                               : Elem<AW4_F16>::load1(w, col + i);
+            }
+        }
+        s[u] = make_float4(v[0], v[1], v[2], v[3]);
+        s[NT * V + u] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+__device__ __forceinline__ void weight8(const float4* s, int chunks, int u, float v[8]) {
+    const float4 a = s[u], b = s[chunks + u];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+constexpr int kNormWarps = 4;       // rows of a block at a time where a warp has a row, at most
+
+// Blocks resident on an SM for that many threads of it.
+template <int NT>
+constexpr int norm_blocks(int threads) {
+    return NT == 32 ? threads / (32 * kNormWarps) : NT < threads ? threads / NT : 1;
+}
+// Forward: 1024 at 64 registers (56 us at 16384 x 4096 bf16; 58 at 768, 64 at 512).  Backward: 512 at 128 (70 us;
+// 96 at 768 and 105 at 1024, where its sums spill).
+constexpr int kNormForward = 1024, kNormBackward = 512;
 
 template <int DT, int NT, int V>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT, kNormBlocks<NT, V>)
-rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, const void* __restrict__ w,
-                        int w_dtype, float eps, const RowsOut y, float* __restrict__ rstd,
-                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ ycodes,
-                        uint8_t* __restrict__ yscales) {
+__global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
+rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, int per_row,
+                        const void* __restrict__ w, int w_dtype, float eps, const RowsOut y,
+                        float* __restrict__ rstd, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                        uint8_t* __restrict__ ycodes, uint8_t* __restrict__ yscales) {
     __shared__ float part[2][NT / 32];
+    extern __shared__ float4 weight_s[];
+    constexpr int kChunks8 = NT * V;
     const int held = NT == 32 ? blockDim.x >> 5 : 1;       // rows of a block at a time
     const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * held;
     int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
-    float wv[V][8];
-#pragma unroll
-    for (int j = 0; j < V; ++j) load_weight8(w, w_dtype, (j * NT + t) * 8, cols, wv[j]);
     Raw8<DT> raw[V];
     if (row < rows)
 #pragma unroll
         for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT>(x, row, (j * NT + t) * 8, cols);
+    stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
     for (int slot = 0; row < rows; row += step, slot ^= 1) {
         Raw8<DT> next[V];
         if (row + step < rows)
@@ -290,17 +333,20 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row
         }
         float s0, s1;
         upk2(ss, s0, s1);
-        const float r = 1.0f / sqrtf(row_sum<NT>(s0 + s1, part, slot) / (float)cols + eps);
+        const float r = inv_sqrt(__fmaf_rn(row_sum<NT>(s0 + s1, part, slot), inv_cols, eps));
         if (t == 0) rstd[row] = r;
+        uint8_t* code_row = codes + row * per_row * 8;
+        uint8_t* scale_row = scales + (row * per_row >> 2);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint32_t u = j * NT + t;
-            float v[8], o[8];
+            const int u = j * NT + t;
+            float v[8], o[8], wv[8];
             widen8<DT>(raw[j], v);
             const A8Block b = a8_block<DT>(raw[j]);
             const uint2 q = a8_encode8(v, b);
+            weight8(weight_s, kChunks8, u, wv);
             vmuls8(o, v, r);
-            vmul8(o, o, wv[j]);
+            vmul8(o, o, wv);
             const Raw8<DT> ry = narrow8<DT>(o);
             A8Block by = {0, 0.0f};
             uint2 qy = make_uint2(0, 0);
@@ -310,13 +356,12 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row
                 qy = a8_encode8(o, by);
             }
             if (u < per_row) {
-                const int64_t at = row * per_row + u;
-                *reinterpret_cast<uint2*>(codes + at * 8) = q;
-                if ((t & 3) == 0) scales[at >> 2] = (uint8_t)b.byte;
-                store_raw8<DT>(y, row, (int)u * 8, cols, ry);
+                *reinterpret_cast<uint2*>(code_row + u * 8) = q;
+                if ((t & 3) == 0) scale_row[u >> 2] = (uint8_t)b.byte;
+                store_raw8<DT>(y, row, u * 8, cols, ry);
                 if (ycodes) {
-                    *reinterpret_cast<uint2*>(ycodes + at * 8) = qy;
-                    if ((t & 3) == 0) yscales[at >> 2] = (uint8_t)by.byte;
+                    *reinterpret_cast<uint2*>(ycodes + row * per_row * 8 + u * 8) = qy;
+                    if ((t & 3) == 0) yscales[(row * per_row + u) >> 2] = (uint8_t)by.byte;
                 }
             }
         }
@@ -336,18 +381,19 @@ struct NormRow {
 
 template <int DT, int NT, int V>
 __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& dy, int64_t row, int t, int cols,
-                                              uint32_t per_row, const uint8_t* codes, const uint8_t* scales,
+                                              int per_row, const uint8_t* codes, const uint8_t* scales,
                                               const float* rstd) {
+    const uint8_t* code_row = codes + row * per_row * 8;
+    const uint8_t* scale_row = scales + (row * per_row >> 2);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const uint32_t u = j * NT + t;
-        const int64_t at = row * per_row + u;
-        n.dy[j] = load_raw8<DT>(dy, row, (int)u * 8, cols);
+        const int u = j * NT + t;
+        n.dy[j] = load_raw8<DT>(dy, row, u * 8, cols);
         n.q[j] = make_uint2(0, 0);
         n.b[j] = 1;
         if (u < per_row) {
-            n.q[j] = __ldcs(reinterpret_cast<const uint2*>(codes + at * 8));
-            n.b[j] = scales[at >> 2];
+            n.q[j] = __ldcs(reinterpret_cast<const uint2*>(code_row + u * 8));
+            n.b[j] = scale_row[u >> 2];
         }
     }
     n.r = rstd[row];
@@ -356,25 +402,26 @@ __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& d
 // dx = r (w dy) - v r^3 mean(v w dy); each block leaves its rows' sum of
 // dy v r in partial[blockIdx.x][cols].
 template <int DT, int NT, int V>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT, kNormBlocks<NT, V>)
-rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, uint32_t per_row,
+__global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormBackward))
+rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols, int per_row,
                          const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                          const float* __restrict__ rstd, const void* __restrict__ w, int w_dtype,
                          const RowsOut dx, float* __restrict__ partial) {
     __shared__ float part[2][NT / 32];
+    extern __shared__ float4 weight_s[];
+    constexpr int kChunks8 = NT * V;
     const int held = NT == 32 ? blockDim.x >> 5 : 1;
     const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * held;
     int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
-    float wv[V][8], acc[V][8];
+    float acc[V][8];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        load_weight8(w, w_dtype, (j * NT + t) * 8, cols, wv[j]);
+    for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
-    }
     NormRow<DT, V> now;
     if (row < rows) load_norm_row<DT, NT, V>(now, dy, row, t, cols, per_row, codes, scales, rstd);
+    stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
     for (int slot = 0; row < rows; row += step, slot ^= 1) {
         NormRow<DT, V> next;
         if (row + step < rows)
@@ -383,33 +430,34 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, uint32_t per_r
         f2 dot2 = pk2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            float d[8], v[8];
+            float d[8], v[8], wv[8];
             widen8<DT>(now.dy[j], d);
             a8_decode8(now.q[j], a8_scale(now.b[j]), v);
             vmul8(d, d, v);
             // behind the last column codes and gradients are zero, but a block may be NaN
-            if ((int)(j * NT + t) * 8 + 8 > cols)
+            if ((j * NT + t) * 8 + 8 > cols)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if ((int)(j * NT + t) * 8 + i >= cols) d[i] = 0.0f;
+                    if ((j * NT + t) * 8 + i >= cols) d[i] = 0.0f;
+            weight8(weight_s, kChunks8, j * NT + t, wv);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2)
-                dot2 = f2_fma(pk2(d[i], d[i + 1]), pk2(wv[j][i], wv[j][i + 1]), dot2);
+            for (int i = 0; i < 8; i += 2) dot2 = f2_fma(pk2(d[i], d[i + 1]), pk2(wv[i], wv[i + 1]), dot2);
             vfmas8(acc[j], r, d, acc[j]);
         }
         float d0, d1;
         upk2(dot2, d0, d1);
-        const float k = r * r * r * (row_sum<NT>(d0 + d1, part, slot) / (float)cols);
+        const float k = r * r * r * (row_sum<NT>(d0 + d1, part, slot) * inv_cols);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint32_t u = j * NT + t;
-            float d[8], v[8];
+            const int u = j * NT + t;
+            float d[8], v[8], wv[8];
             widen8<DT>(now.dy[j], d);
             a8_decode8(now.q[j], a8_scale(now.b[j]), v);
-            vmul8(d, d, wv[j]);
+            weight8(weight_s, kChunks8, u, wv);
+            vmul8(d, d, wv);
             vmuls8(d, d, r);
             vfmas8(d, -k, v, d);
-            if (u < per_row) store_raw8<DT>(dx, row, (int)u * 8, cols, narrow8<DT>(d));
+            if (u < per_row) store_raw8<DT>(dx, row, u * 8, cols, narrow8<DT>(d));
         }
         now = next;
     }
@@ -496,16 +544,15 @@ static RowsIn rows_in(const void* p, int64_t rows, int64_t cols, int64_t ld, int
 }
 static RowsOut rows_out(void* p, int64_t ld, int dtype) { return {static_cast<char*>(p), ld, vec_ok(p, ld, dtype)}; }
 
-// A row's threads and chunks: one chunk a thread where 512 threads cover the row (the sums and weights of two
-// chunks take the registers of half the warps), a warp without a barrier up to 256 columns.
+// A row's threads and chunks of eight.
 template <typename F>
 static int32_t norm_shape(int64_t cols, F f) {
     using std::integral_constant;
     if (cols <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
-    if (cols <= 512) return f(integral_constant<int, 64>(), integral_constant<int, 1>());
-    if (cols <= 1024) return f(integral_constant<int, 128>(), integral_constant<int, 1>());
-    if (cols <= 2048) return f(integral_constant<int, 256>(), integral_constant<int, 1>());
-    if (cols <= 4096) return f(integral_constant<int, 512>(), integral_constant<int, 1>());
+    if (cols <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 2>());
+    if (cols <= 1024) return f(integral_constant<int, 64>(), integral_constant<int, 2>());
+    if (cols <= 2048) return f(integral_constant<int, 128>(), integral_constant<int, 2>());
+    if (cols <= 4096) return f(integral_constant<int, 256>(), integral_constant<int, 2>());
     if (cols <= 8192) return f(integral_constant<int, 512>(), integral_constant<int, 2>());
     return f(integral_constant<int, 1024>(), integral_constant<int, 2>());
 }
@@ -519,17 +566,28 @@ static int32_t by_dtype(int dtype, F f) {
 
 constexpr int64_t kNormCols = 16384;
 
-// Where a warp has a row: warps of a block, one for each SM's share of few rows, eight at most.
+// Where a warp has a row: warps of a block, one for each SM's share of few rows.
 static int norm_warps(int device, int64_t rows) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(8, rows / sm_count(device)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(kNormWarps, rows / sm_count(device)));
 }
 
 // Resident blocks, or as many as have a row: of the backward kernel also the rows of its partial sums.
-template <int NT, int V>
-static int norm_grid(int device, int64_t rows) {
+template <int NT>
+static int norm_grid(int device, int64_t rows, int threads) {
     const int held = NT == 32 ? norm_warps(device, rows) : 1;
-    const int resident = NT == 32 ? kNormBlocks<NT, V> * 8 / held : kNormBlocks<NT, V>;
+    const int resident = NT == 32 ? threads / (32 * held) : norm_blocks<NT>(threads);
     return (int)std::min<int64_t>((rows + held - 1) / held, (int64_t)sm_count(device) * resident);
+}
+template <int NT>
+static int norm_threads(int device, int64_t rows) {
+    return NT == 32 ? 32 * norm_warps(device, rows) : NT;
+}
+
+template <typename K>
+static int32_t norm_smem(K kernel, int bytes) {
+    if (bytes <= 32 * 1024) return AW4_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e == cudaSuccess ? (int32_t)AW4_OK : fail(AW4_ERR_CUDA, "rms_norm: %s", cudaGetErrorString(e));
 }
 
 }  // namespace aw4
@@ -583,7 +641,7 @@ extern "C" int32_t aw4_swiglu_forward(const void* gate, const void* up, int32_t 
     const uint32_t per_row = chunks_per_row(cols);
     const RowsIn g = rows_in(gate, rows, cols, ld_gate, dtype), u = rows_in(up, rows, cols, ld_up, dtype);
     const RowsOut o = rows_out(h, cols, dtype);
-    const unsigned grid = run_grid(rows * per_row, kGluRun);
+    const unsigned grid = run_grid(rows * per_row, 32 * kGluForward);
     return by_dtype(dtype, [&](auto dt) {
         if (hcodes)
             swiglu_forward_kernel<dt.value, true><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
@@ -609,7 +667,7 @@ extern "C" int32_t aw4_swiglu_backward(const void* dh, int32_t dtype, int64_t ro
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
         swiglu_backward_kernel<dt.value>
-            <<<run_grid(rows * per_row, kGluRun), kA8Threads, 0, (cudaStream_t)stream>>>(
+            <<<run_grid(rows * per_row, 32 * kGluBackward), kA8Threads, 0, (cudaStream_t)stream>>>(
                 rows_in(dh, rows, cols, ld_dh, dtype), rows, (int)cols, per_row, gcodes, gscales, ucodes, uscales,
                 rows_out(dgate, ld_out, dtype), rows_out(dup, ld_out, dtype));
         return launched("swiglu_backward");
@@ -634,11 +692,13 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
     const uint32_t per_row = chunks_per_row(cols);
     return by_dtype(dtype, [&](auto dt) {
         return norm_shape(cols, [&](auto nt, auto v) {
-            rms_norm_forward_kernel<dt.value, nt.value, v.value>
-                <<<norm_grid<nt.value, v.value>(device, rows),
-                   nt.value == 32 ? 32 * norm_warps(device, rows) : nt.value, 0, (cudaStream_t)stream>>>(
-                    rows_in(x, rows, cols, ld, dtype), rows, (int)cols, per_row, weight, weight_dtype, eps,
-                    rows_out(y, cols, dtype), rstd, codes, scales, ycodes, yscales);
+            auto kernel = rms_norm_forward_kernel<dt.value, nt.value, v.value>;
+            const int bytes = nt.value * v.value * 32;
+            if (const int32_t rc = norm_smem(kernel, bytes)) return rc;
+            kernel<<<norm_grid<nt.value>(device, rows, kNormForward), norm_threads<nt.value>(device, rows), bytes,
+                     (cudaStream_t)stream>>>(rows_in(x, rows, cols, ld, dtype), rows, (int)cols, 1.0f / (float)cols,
+                                             (int)per_row, weight, weight_dtype, eps, rows_out(y, cols, dtype), rstd,
+                                             codes, scales, ycodes, yscales);
             return launched("rms_norm_forward");
         });
     });
@@ -647,9 +707,9 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
 extern "C" uint64_t aw4_rms_norm_backward_workspace(int64_t rows, int64_t cols, int32_t device) {
     if (rows <= 0 || cols <= 0 || cols > kNormCols) return 0;
     int grid = 0;
-    norm_shape(cols, [&](auto nt, auto v) {
-        grid = norm_grid<nt.value, v.value>(device, rows);
-        return AW4_OK;
+    norm_shape(cols, [&](auto nt, auto) {
+        grid = norm_grid<nt.value>(device, rows, kNormBackward);
+        return (int32_t)AW4_OK;
     });
     return (uint64_t)grid * cols * sizeof(float);
 }
@@ -683,11 +743,13 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
     int grid = 0;
     const int32_t rc = by_dtype(dtype, [&](auto dt) {
         return norm_shape(cols, [&](auto nt, auto v) {
-            grid = norm_grid<nt.value, v.value>(device, rows);
-            rms_norm_backward_kernel<dt.value, nt.value, v.value>
-                <<<grid, nt.value == 32 ? 32 * norm_warps(device, rows) : nt.value, 0, s>>>(
-                    rows_in(dy, rows, cols, ld, dtype), rows, (int)cols, per_row, codes, scales, rstd, weight,
-                    weight_dtype, rows_out(dx, cols, dtype), workspace);
+            auto kernel = rms_norm_backward_kernel<dt.value, nt.value, v.value>;
+            const int bytes = nt.value * v.value * 32;
+            if (const int32_t rc = norm_smem(kernel, bytes)) return rc;
+            grid = norm_grid<nt.value>(device, rows, kNormBackward);
+            kernel<<<grid, norm_threads<nt.value>(device, rows), bytes, s>>>(
+                rows_in(dy, rows, cols, ld, dtype), rows, (int)cols, 1.0f / (float)cols, (int)per_row, codes, scales,
+                rstd, weight, weight_dtype, rows_out(dx, cols, dtype), workspace);
             return launched("rms_norm_backward");
         });
     });

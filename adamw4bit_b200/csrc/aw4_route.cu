@@ -15,9 +15,9 @@
 // A row that is not valid, or whose logits are all -inf, takes no part:
 // choices -1, weights 0, gradient 0, no count.
 //
-// Counts are integers; the sums of p go through registers, then blocks'
-// partial sums, then one block, each in a fixed order, so a repeated call
-// gives the same bits.
+// Counts are integers; the sums of p go through registers and shared memory in
+// a fixed order, then as whole numbers from block to block, so a repeated
+// call gives the same bits.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -50,9 +50,11 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return v;
 }
 
-__device__ __forceinline__ float exp_near(float x) {       // 2^-22 of the value, and 2^-24 |x| of it
+// exp(l - top): 2^-22 of the value, and 2^-24 |l - top| of it.  The difference comes
+// first: products of logits near the type's limits would overflow.
+__device__ __forceinline__ float exp_from(float l, float top) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((l - top) * 1.44269504f));
     return r;
 }
 
@@ -64,39 +66,31 @@ __device__ __forceinline__ uint32_t order_key(float l) {
     const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
     return l != l ? 0xffffffffu : k;
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
-    if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
-    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
-struct Pick {
-    float value;
-    int expert;       // -1: none left above -inf
-};
-
 // Takes a row's logits from the largest down.  float32: the largest key left by a scan and
 // shuffles, then the lowest lane and place that has it by a ballot.
 template <int DT, int L, int V, bool kPacked = DT != AW4_F32>
 struct Picker {
     uint32_t key[V];
-    __device__ __forceinline__ Picker(const float l[V], int lane, int experts, bool ok) {
+    __device__ __forceinline__ Picker(const float l[V], int) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = ok && expert_of<L>(lane, i) < experts ? order_key(l[i]) : 0u;
+        for (int i = 0; i < V; ++i) key[i] = order_key(l[i]);
     }
-    __device__ __forceinline__ Pick next(int lane) {
+    // The next key and the expert that has it; a key of 0 has none.
+    __device__ __forceinline__ uint32_t next(int lane, int& at) {
         uint32_t best = key[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = max(best, key[i]);
         best = lanes_max<L>(best);
-        int at = 0x7fffffff;
+        at = 0x7fffffff;
 #pragma unroll
         for (int i = V - 1; i >= 0; --i)
             if (key[i] == best) at = expert_of<L>(lane, i);
         if constexpr (V == 8) {
             // lanes hold ascending experts: the first lane that has it
             const uint32_t here = (threadIdx.x & 31) & ~(L - 1);
-            const uint32_t has = __ballot_sync(0xffffffffu, at != 0x7fffffff) >> here;
-            at = __shfl_sync(0xffffffffu, at, here + (L == 32 ? __ffs(has) : __ffs(has & ((1u << (L & 31)) - 1))) - 1);
+            uint32_t has = __ballot_sync(0xffffffffu, at != 0x7fffffff) >> here;
+            if constexpr (L < 32) has &= (1u << L) - 1;
+            at = __shfl_sync(0xffffffffu, at, here + __ffs(has) - 1);
         } else {
 #pragma unroll
             for (int o = L / 2; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
@@ -104,29 +98,33 @@ struct Picker {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (at == expert_of<L>(lane, i)) key[i] = 0;
-        return {key_value(best), best > kKeyNegInf ? at : -1};
+        return best;
+    }
+    static __device__ __forceinline__ bool some(uint32_t best) { return best > kKeyNegInf; }
+    static __device__ __forceinline__ int expert(uint32_t, int at) { return at; }
+    static __device__ __forceinline__ float value(uint32_t k) {
+        if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+        return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
     }
 };
 
 // 16-bit logits: their order in the upper half of a word and the index, counted
 // down, in the lower.  Words are then all different and one maximum gives both.
-// Eight of a lane are sorted once; a lane's largest is then its first.
+// Eight of a lane are sorted once (Batcher's odd-even merge); a lane's largest is then its first.
 template <int DT, int L, int V>
 struct Picker<DT, L, V, true> {
     uint32_t key[V];
-    static constexpr uint32_t kNegInf = DT == AW4_BF16 ? 0x007fu : 0x03ffu;
 
-    __device__ __forceinline__ Picker(const float l[V], int lane, int experts, bool ok) {
+    __device__ __forceinline__ Picker(const float l[V], int lane) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int e = expert_of<L>(lane, i);
             const float z = l[i] + 0.0f;
             const uint32_t u = DT == AW4_BF16 ? __float_as_uint(z)
                                               : (uint32_t)__half_as_ushort(__float2half_rn(z)) << 16;
-            const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-            key[i] = !(ok && e < experts) ? 0u
-                     : l[i] != l[i]       ? 0xffff0000u | (0xffffu - e)
-                                          : (k & 0xffff0000u) | (0xffffu - e);
+            uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+            k = l[i] != l[i] ? 0xffffffffu : k;
+            key[i] = (k & 0xffff0000u) | (0xffffu - e);
         }
         if constexpr (V == 8) {
             constexpr int kA[19] = {0, 2, 4, 6, 0, 1, 4, 5, 1, 5, 0, 1, 2, 3, 2, 3, 1, 3, 5};
@@ -139,7 +137,7 @@ struct Picker<DT, L, V, true> {
             }
         }
     }
-    __device__ __forceinline__ Pick next(int) {
+    __device__ __forceinline__ uint32_t next(int, int&) {
         uint32_t mine = key[0];
         if constexpr (V != 8)
 #pragma unroll
@@ -154,60 +152,68 @@ struct Picker<DT, L, V, true> {
             for (int i = 0; i < V; ++i)
                 if (key[i] == best) key[i] = 0;
         }
+        return best;
+    }
+    static __device__ __forceinline__ bool some(uint32_t best) {
+        return (best >> 16) > (DT == AW4_BF16 ? 0x007fu : 0x03ffu);         // above -inf
+    }
+    static __device__ __forceinline__ int expert(uint32_t best, int) { return (int)(0xffffu - (best & 0xffffu)); }
+    static __device__ __forceinline__ float value(uint32_t best) {
         const uint32_t top = best >> 16;
-        float value;
-        if (top == 0xffffu) {
-            value = __uint_as_float(0x7fc00000u);
-        } else {
-            const uint32_t u = (top & 0x8000u) ? top & 0x7fffu : ~top & 0xffffu;
-            value = DT == AW4_BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
-        }
-        return {value, top > kNegInf ? (int)(0xffffu - (best & 0xffffu)) : -1};
+        if (top == 0xffffu) return __uint_as_float(0x7fc00000u);
+        const uint32_t u = (top & 0x8000u) ? top & 0x7fffu : ~top & 0xffffu;
+        return DT == AW4_BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
     }
 };
 
+// A row's logits, -inf in the place of those that take no part.
 template <int DT, int L, int V>
 __device__ __forceinline__ void load_logits(const RowsIn& logits, int64_t row, int lane, int experts, bool in,
                                             float l[V]) {
 #pragma unroll
     for (int c = 0; c < V / 8; ++c)
         widen8<DT>(load_raw8<DT>(logits, in ? row : 0, (c * L + lane) * 8, in ? experts : 0), l + c * 8);
+    if (!in || experts < L * V)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (!in || expert_of<L>(lane, i) >= experts) l[i] = -INFINITY;
 }
 
 // Threads of a forward block: a block an SM, its sums over rows in registers.
 template <int V>
 constexpr int kRouteThreads = V == 8 ? 1024 : V == 16 ? 512 : 256;
 
-// Balance loss from all experts' sums; called by a whole block.
-template <int T>
-__device__ __forceinline__ void finish_balance(float mine, int n, int experts, int k, float* scratch, float* balance) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float s = 0.0f;
-        for (int i = 0; i < T / 32; ++i) s += scratch[i];
-        *balance = n ? s * ((float)experts / (float)k) / (float)n / (float)n : 0.0f;
-    }
+// What the blocks of a call add up, zero before it.  The sums of p are whole
+// numbers of 2^-32, so that the order of the additions does not matter; a
+// block's sum that is no number is counted instead.
+struct RouteTotals {
+    unsigned arrived;
+    int valid_rows, not_numbers, pad;
+    // then unsigned long long sum[experts], int count[experts]
+};
+constexpr float kRouteUnit = 4294967296.0f;
+
+__host__ __device__ constexpr int64_t route_totals_bytes(int experts) {
+    return (int64_t)sizeof(RouteTotals) + 12 * (int64_t)experts;
 }
 
 template <int DT, int L, int V>
 __global__ void __launch_bounds__(kRouteThreads<V>, 1)
 route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, const uint8_t* __restrict__ valid,
                      bool renormalize, float* __restrict__ weights, int32_t* __restrict__ chosen,
-                     float2* __restrict__ stats, float* __restrict__ psum, int32_t* __restrict__ pcount,
-                     int32_t* __restrict__ counts, float* __restrict__ balance) {
+                     float2* __restrict__ stats, RouteTotals* __restrict__ totals, int32_t* __restrict__ counts,
+                     int32_t* __restrict__ valid_rows, float* __restrict__ balance) {
     constexpr int kThreads = kRouteThreads<V>, kRows = kThreads / L;
     extern __shared__ int32_t smem[];
+    __shared__ float scratch[kThreads / 32];
+    __shared__ int is_last;
     int32_t* count = smem;                                            // [experts + 1], the last: valid rows
-    float* sums = reinterpret_cast<float*>(count + experts + 1);      // [experts]
-    float* weight_s = sums + experts;                                 // [rows][k]
-    int32_t* chosen_s = reinterpret_cast<int32_t*>(weight_s + kRows * k);
+    uint32_t* key_s = reinterpret_cast<uint32_t*>(count + experts + 1);       // [rows][k]
+    int32_t* chosen_s = reinterpret_cast<int32_t*>(key_s + kRows * k);
     for (int i = threadIdx.x; i <= experts; i += kThreads) count[i] = 0;
     __syncthreads();
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
-    float* my_weight = weight_s + group * k;
+    uint32_t* my_key = key_s + group * k;
     int32_t* my_chosen = chosen_s + group * k;
     float acc[V];
 #pragma unroll
@@ -219,42 +225,55 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
         bool ok = in && (!valid || valid[row]);
         float l[V];
         load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
-        Picker<DT, L, V> picker(l, lane, experts, ok);
-        Pick pick = picker.next(lane);
-        ok = ok && pick.expert >= 0;
-        const float top = pick.value;
+        using P = Picker<DT, L, V>;
+        P picker(l, lane);
+        // the k largest, kept by the lanes in turn
+        int at = 0;
+        const uint32_t first = picker.next(lane, at);
+        if (lane == 0) {
+            my_key[0] = first;
+            if constexpr (DT == AW4_F32) my_chosen[0] = at;
+        }
+#pragma unroll 2
+        for (int j = 1; j < k; ++j) {
+            const uint32_t best = picker.next(lane, at);
+            if (lane == j % L) {
+                my_key[j] = best;
+                if constexpr (DT == AW4_F32) my_chosen[j] = at;
+            }
+        }
+        ok = ok && P::some(first);
+        const float top = P::value(first);
         float part = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = ok && expert_of<L>(lane, i) < experts ? exp_near(l[i] - top) : 0.0f;
+            l[i] = exp_from(l[i], top);
             part += l[i];
         }
         const float total = lanes_sum<L>(part);
         const float inv = ok ? 1.0f / total : 0.0f;
+        if (ok)
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = ok ? __fmaf_rn(l[i], inv, acc[i]) : acc[i];
-        // the choices, by the lanes in turn; all lanes know each
-        float chosen_sum = 0.0f;
-        for (int j = 0; j < k; ++j) {
-            const bool take = ok && pick.expert >= 0;
-            const float w = take ? exp_near(pick.value - top) : 0.0f;
-            chosen_sum += w;
-            if (lane == j % L) {
-                my_weight[j] = w;
-                my_chosen[j] = take ? pick.expert : -1;
-                if (take) atomicAdd(&count[pick.expert], 1);
-            }
-            if (j + 1 < k) pick = picker.next(lane);
+            for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(l[i], inv, acc[i]);
+        float scale = inv;
+        if (renormalize) {
+            float chosen_sum = 0.0f;
+            for (int j = lane; j < k; j += L)
+                if (ok && P::some(my_key[j])) chosen_sum += exp_from(P::value(my_key[j]), top);
+            chosen_sum = lanes_sum<L>(chosen_sum);
+            scale = ok ? 1.0f / chosen_sum : 0.0f;
         }
-        const float scale = !ok ? 0.0f : renormalize ? 1.0f / chosen_sum : inv;
         if (in) {
             if (lane == 0) {
                 stats[row] = make_float2(top, inv);
                 if (ok) atomicAdd(&count[experts], 1);
             }
             for (int j = lane; j < k; j += L) {       // its own choices
-                weights[row * k + j] = my_weight[j] * scale;
-                chosen[row * k + j] = my_chosen[j];
+                const bool take = ok && P::some(my_key[j]);
+                const int e = take ? P::expert(my_key[j], DT == AW4_F32 ? my_chosen[j] : 0) : -1;
+                weights[row * k + j] = take ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
+                chosen[row * k + j] = e;
+                if (take) atomicAdd(&count[e], 1);
             }
         }
     }
@@ -264,65 +283,56 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
 #pragma unroll
         for (int o = 16; o >= L; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
     __syncthreads();
-    float* warp_sums = weight_s;                      // [kThreads / 32][V L]: the choices are out
+    float* warp_sums = reinterpret_cast<float*>(key_s);       // [kThreads / 32][V L]: the choices are out
     if ((threadIdx.x & 31) < L)
 #pragma unroll
         for (int i = 0; i < V; ++i) warp_sums[(threadIdx.x >> 5) * (V * L) + expert_of<L>(lane, i)] = acc[i];
     __syncthreads();
+    unsigned long long* sum_t = reinterpret_cast<unsigned long long*>(totals + 1);
+    int* count_t = reinterpret_cast<int*>(sum_t + experts);
+    const bool alone = gridDim.x == 1;
+    float mine = 0.0f;
     for (int e = threadIdx.x; e < experts; e += kThreads) {
         float s = 0.0f;
 #pragma unroll 8
         for (int w = 0; w < kThreads / 32; ++w) s += warp_sums[w * (V * L) + e];
-        sums[e] = s;
-    }
-    __syncthreads();
-    if (gridDim.x == 1) {
-        float mine = 0.0f;
-        for (int e = threadIdx.x; e <= experts; e += kThreads) {
+        if (alone) {
             counts[e] = count[e];
-            if (e < experts) mine = __fmaf_rn((float)count[e], sums[e], mine);
+            mine = __fmaf_rn((float)count[e], s, mine);
+        } else {
+            if (count[e]) atomicAdd(&count_t[e], count[e]);
+            if (s == s) atomicAdd(&sum_t[e], (unsigned long long)(s * kRouteUnit));
+            else atomicAdd(&totals->not_numbers, 1);
         }
-        finish_balance<kThreads>(mine, count[experts], experts, k, warp_sums, balance);
-        return;
     }
-    for (int i = threadIdx.x; i < experts; i += kThreads) psum[(int64_t)blockIdx.x * experts + i] = sums[i];
-    for (int i = threadIdx.x; i <= experts; i += kThreads)
-        pcount[(int64_t)blockIdx.x * (experts + 1) + i] = count[i];
-}
-
-// One block: counts, the number of valid rows and the balance loss from the blocks' parts.  1024 / C threads
-// share an expert's parts, C the experts rounded up to a power of two.
-__global__ void __launch_bounds__(1024)
-route_finish_kernel(const float* __restrict__ psum, const int32_t* __restrict__ pcount, int parts, int experts,
-                    int log_c, int k, int32_t* __restrict__ counts, float* __restrict__ balance) {
-    __shared__ float sum_s[1024], scratch[32];
-    __shared__ int count_s[1024], valid_rows;
-    const int c = 1 << log_c, e = threadIdx.x & (c - 1), slice = threadIdx.x >> log_c, slices = 1024 >> log_c;
-    if (threadIdx.x == 0) valid_rows = 0;
-    float s = 0.0f;
-    int n = 0;
-    if (e < experts)
-#pragma unroll 8
-        for (int p = slice; p < parts; p += slices) {
-            s += psum[(int64_t)p * experts + e];
-            n += pcount[(int64_t)p * (experts + 1) + e];
+    int n = count[experts], bad = 0;
+    if (!alone) {
+        if (threadIdx.x == 0 && n) atomicAdd(&totals->valid_rows, n);
+        // the block that arrives last has every block's additions before it
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) is_last = atomicAdd(&totals->arrived, 1u) == gridDim.x - 1;
+        __syncthreads();
+        if (!is_last) return;
+        __threadfence();
+        n = __ldcg(&totals->valid_rows);
+        bad = __ldcg(&totals->not_numbers);
+        for (int e = threadIdx.x; e < experts; e += kThreads) {
+            const int c = __ldcg(&count_t[e]);
+            counts[e] = c;
+            mine = __fmaf_rn((float)c, (float)__ldcg(&sum_t[e]) / kRouteUnit, mine);
         }
-    sum_s[threadIdx.x] = s;
-    count_s[threadIdx.x] = n;
-    __syncthreads();
-    for (int p = threadIdx.x; p < parts; p += 1024) atomicAdd(&valid_rows, pcount[(int64_t)p * (experts + 1) + experts]);
-    float mine = 0.0f;
-    if (slice == 0 && e < experts) {
-        for (int i = 1; i < slices; ++i) {
-            s += sum_s[(i << log_c) + e];
-            n += count_s[(i << log_c) + e];
-        }
-        counts[e] = n;
-        mine = (float)n * s;
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = mine;
     __syncthreads();
-    if (threadIdx.x == 0) counts[experts] = valid_rows;
-    finish_balance<1024>(mine, valid_rows, experts, k, scratch, balance);
+    if (threadIdx.x == 0) {
+        float s = bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+        for (int i = 0; i < kThreads / 32; ++i) s += scratch[i];
+        *balance = n ? s * ((float)experts / (float)k) / (float)n / (float)n : 0.0f;
+        *valid_rows = n;
+    }
 }
 
 constexpr int kRouteBackThreads = 256;
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kRouteBackThreads)
 route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, bool renormalize,
                       const float* __restrict__ weights, const int32_t* __restrict__ chosen,
                       const float2* __restrict__ stats, const int32_t* __restrict__ counts,
-                      const float* __restrict__ dweights, const float* __restrict__ dbalance,
+                      const int32_t* __restrict__ valid_rows, const float* __restrict__ dweights, const float* __restrict__ dbalance,
                       const RowsOut dlogits) {
     constexpr int kRows = kRouteBackThreads / L;
     // t_j at its expert's place, zero elsewhere: written and cleared by the lanes that have the choices
@@ -342,7 +352,7 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
 #pragma unroll
     for (int i = 0; i < V; ++i) mine[expert_of<L>(lane, i)] = 0.0f;
     __syncwarp();
-    const float n = fmaxf((float)counts[experts], 1.0f);
+    const float n = fmaxf((float)*valid_rows, 1.0f);
     const float unit = dbalance ? *dbalance * ((float)experts / (float)k) / n / n : 0.0f;
     float share[V];
 #pragma unroll
@@ -356,24 +366,39 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         const bool in = row < rows;
         const float2 st = in ? stats[row] : make_float2(0.0f, 0.0f);
         const bool ok = st.y != 0.0f;             // a NaN row is a valid one
+        // a lane's first choice is loaded with the logits
+        const int picks = dweights && in ? k : 0;
+        int at = -1;
+        float w = 0.0f, d = 0.0f;
+        if (lane < picks) {
+            at = chosen[row * k + lane];
+            w = weights[row * k + lane];
+            d = dweights[row * k + lane];
+        }
         float l[V];
         load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
-        const bool picks = dweights && ok;
         float inner = 0.0f;
-        if (picks)
-            for (int j = lane; j < k; j += L)
-                if (chosen[row * k + j] >= 0)
-                    inner = __fmaf_rn(weights[row * k + j], dweights[row * k + j], inner);
-        inner = lanes_sum<L>(inner);
-        if (picks)
-            for (int j = lane; j < k; j += L) {
-                const int at = chosen[row * k + j];
-                if (at >= 0) mine[at] = weights[row * k + j] * (dweights[row * k + j] - (renormalize ? inner : 0.0f));
+        for (int j = lane; j < picks; j += L) {
+            if (j != lane) {
+                at = chosen[row * k + j];
+                w = weights[row * k + j];
+                d = dweights[row * k + j];
             }
+            if (at >= 0) inner = __fmaf_rn(w, d, inner);
+        }
+        inner = lanes_sum<L>(inner);
+        for (int j = lane; j < picks; j += L) {
+            if (k > L) {
+                at = chosen[row * k + j];
+                w = weights[row * k + j];
+                d = dweights[row * k + j];
+            }
+            if (at >= 0) mine[at] = w * (d - (renormalize ? inner : 0.0f));
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = ok && expert_of<L>(lane, i) < experts ? exp_near(l[i] - st.x) * st.y : 0.0f;
+            l[i] = ok ? exp_from(l[i], st.x) * st.y : 0.0f;
             sum = __fmaf_rn(l[i], share[i], sum);
         }
         sum = lanes_sum<L>(sum);
@@ -382,11 +407,10 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
 #pragma unroll
         for (int i = 0; i < V; ++i) l[i] = __fmaf_rn(l[i], share[i] - off, mine[expert_of<L>(lane, i)]);
         __syncwarp();
-        if (picks)
-            for (int j = lane; j < k; j += L) {
-                const int at = chosen[row * k + j];
-                if (at >= 0) mine[at] = 0.0f;
-            }
+        for (int j = lane; j < picks; j += L) {
+            if (k > L) at = chosen[row * k + j];
+            if (at >= 0) mine[at] = 0.0f;
+        }
         if (in)
 #pragma unroll
             for (int c = 0; c < V / 8; ++c)
@@ -456,67 +480,65 @@ using namespace aw4;
 
 extern "C" uint64_t aw4_route_forward_workspace(int64_t rows, int32_t experts, int32_t device) {
     if (rows <= 0 || experts < 1 || experts > AW4_ROUTE_MAX_EXPERTS) return 0;
-    return (uint64_t)route_grid(device, rows, experts) * (2 * experts + 1) * 4;
+    return route_grid(device, rows, experts) == 1 ? 0 : (uint64_t)route_totals_bytes(experts);
 }
 
 extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
                                      int32_t k, const uint8_t* valid, int32_t renormalize, float* weights,
-                                     int32_t* chosen, float* stats, int32_t* counts, float* balance,
-                                     void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
+                                     int32_t* chosen, float* stats, int32_t* counts, int32_t* valid_rows,
+                                     float* balance, void* workspace, int64_t workspace_bytes, int32_t device,
+                                     void* stream) {
     if (const int32_t rc = check_route("aw4_route_forward", dtype, rows, experts, k)) return rc;
-    if (!counts || !balance) return fail(AW4_ERR_INVALID, "aw4_route_forward: null buffer");
+    if (!counts || !valid_rows || !balance) return fail(AW4_ERR_INVALID, "aw4_route_forward: null buffer");
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     cudaStream_t s = (cudaStream_t)stream;
     if (rows == 0) {
-        cudaError_t e = cudaMemsetAsync(counts, 0, (experts + 1) * 4, s);
+        cudaError_t e = cudaMemsetAsync(counts, 0, experts * 4, s);
+        if (e == cudaSuccess) e = cudaMemsetAsync(valid_rows, 0, 4, s);
         if (e == cudaSuccess) e = cudaMemsetAsync(balance, 0, 4, s);
         return e == cudaSuccess ? AW4_OK : fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
     }
     if (!logits || !weights || !chosen || !stats || (uintptr_t)stats % 8)
         return fail(AW4_ERR_INVALID, "aw4_route_forward: null or misaligned buffer");
     const int grid = route_grid(device, rows, experts);
-    if (!workspace || workspace_bytes < (int64_t)grid * (2 * experts + 1) * 4)
-        return fail(AW4_ERR_INVALID, "aw4_route_forward: workspace of %lld bytes is too small",
-                    (long long)workspace_bytes);
-    float* psum = static_cast<float*>(workspace);
-    int32_t* pcount = reinterpret_cast<int32_t*>(psum + (int64_t)grid * experts);
-    const int32_t rc = route_by_dtype(dtype, [&](auto dt) {
+    if (grid > 1) {
+        if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < route_totals_bytes(experts))
+            return fail(AW4_ERR_INVALID, "aw4_route_forward: workspace of %lld bytes is too small or misaligned",
+                        (long long)workspace_bytes);
+        const cudaError_t e = cudaMemsetAsync(workspace, 0, route_totals_bytes(experts), s);
+        if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
+    }
+    return route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
             constexpr int kThreads = kRouteThreads<v.value>;
             // choices of the rows in work, later the warps' sums
             const int choices = std::max(2 * (kThreads / lanes.value) * k, kThreads / 32 * v.value * lanes.value);
             auto kernel = route_forward_kernel<dt.value, lanes.value, v.value>;
-            const int bytes = (2 * experts + 1 + choices) * 4;
-            if (bytes > 48 * 1024) {
+            const int bytes = (experts + 1 + choices) * 4;
+            if (bytes > 40 * 1024) {
                 const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
                 if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
             }
-            kernel<<<grid, kThreads, bytes, s>>>(
-                    route_rows(logits, rows, experts, ld, dtype), rows, experts, k, valid, renormalize != 0, weights,
-                    chosen, reinterpret_cast<float2*>(stats), psum, pcount, counts, balance);
+            kernel<<<grid, kThreads, bytes, s>>>(route_rows(logits, rows, experts, ld, dtype), rows, experts, k, valid,
+                                                 renormalize != 0, weights, chosen, reinterpret_cast<float2*>(stats),
+                                                 static_cast<RouteTotals*>(workspace), counts, valid_rows, balance);
             note_launch();
             const cudaError_t e = cudaGetLastError();
             return e == cudaSuccess ? (int32_t)AW4_OK
                                     : fail(AW4_ERR_CUDA, "route_forward launch: %s", cudaGetErrorString(e));
         });
     });
-    if (rc || grid == 1) return rc;
-    int log_c = 0;
-    while ((1 << log_c) < experts) ++log_c;
-    route_finish_kernel<<<1, 1024, 0, s>>>(psum, pcount, grid, experts, log_c, k, counts, balance);
-    note_launch();
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? AW4_OK : fail(AW4_ERR_CUDA, "route_finish launch: %s", cudaGetErrorString(e));
 }
 
 extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
                                       int32_t k, int32_t renormalize, const float* weights, const int32_t* chosen,
-                                      const float* stats, const int32_t* counts, const float* dweights,
-                                      const float* dbalance, void* dlogits, int32_t device, void* stream) {
+                                      const float* stats, const int32_t* counts, const int32_t* valid_rows,
+                                      const float* dweights, const float* dbalance, void* dlogits, int32_t device,
+                                      void* stream) {
     if (const int32_t rc = check_route("aw4_route_backward", dtype, rows, experts, k)) return rc;
     if (rows == 0) return AW4_OK;
-    if (!logits || !weights || !chosen || !stats || !counts || !dlogits || (uintptr_t)stats % 8)
+    if (!logits || !weights || !chosen || !stats || !counts || !valid_rows || !dlogits || (uintptr_t)stats % 8)
         return fail(AW4_ERR_INVALID, "aw4_route_backward: null or misaligned buffer");
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
@@ -527,7 +549,7 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
             route_backward_kernel<dt.value, lanes.value, v.value>
                 <<<grid, kRouteBackThreads, 0, (cudaStream_t)stream>>>(
                     route_rows(logits, rows, experts, ld, dtype), rows, experts, k, renormalize != 0, weights, chosen,
-                    reinterpret_cast<const float2*>(stats), counts, dweights, dbalance,
+                    reinterpret_cast<const float2*>(stats), counts, valid_rows, dweights, dbalance,
                     RowsOut{static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)});
             note_launch();
             const cudaError_t e = cudaGetLastError();

@@ -40,15 +40,15 @@ class Routed(NamedTuple):
 
 
 class Routing(NamedTuple):
-    """The outputs of ``route_forward`` and what its backward call reads: the logits as they were, each
-    token's largest logit and 1 / sum exp, and the counts with the number of valid tokens behind them."""
+    """The outputs of ``route_forward`` and what its backward call reads: the logits as they were, and
+    ``stats``, two float32 for each token (its largest logit, 1 / sum exp), the number of valid tokens
+    behind them."""
     weights: torch.Tensor
     experts: torch.Tensor
     counts: torch.Tensor
     balance_loss: torch.Tensor
     logits: torch.Tensor
     stats: torch.Tensor
-    totals: torch.Tensor
     k: int
     renormalize: bool
 
@@ -76,16 +76,17 @@ def route_forward(logits: torch.Tensor, k: int, valid: torch.Tensor | None = Non
         valid = valid.contiguous()
     weights = logits.new_empty((*lead, k), dtype=torch.float32)
     chosen = logits.new_empty((*lead, k), dtype=torch.int32)
-    stats = weights.new_empty((rows, 2))
-    totals = chosen.new_empty(experts + 1)
+    counts = chosen.new_empty(experts)
     balance = weights.new_empty(())
     nbytes = _workspace(rows, experts, dev)
-    ws = logits.new_empty(nbytes, dtype=torch.uint8)
+    # statistics, the number of valid rows, and behind them the call's workspace
+    stats = weights.new_empty(2 * rows + 2 + nbytes // 4)
+    at = stats.data_ptr()
     N.check(N.lib().aw4_route_forward(src.data_ptr(), code, rows, experts, ld, k, N.ptr(valid), int(renormalize),
-                                      weights.data_ptr(), chosen.data_ptr(), stats.data_ptr(), totals.data_ptr(),
-                                      balance.data_ptr(), ws.data_ptr(), nbytes, dev, N.stream_of(dev)),
+                                      weights.data_ptr(), chosen.data_ptr(), at, counts.data_ptr(), at + 8 * rows,
+                                      balance.data_ptr(), at + 8 * rows + 8, nbytes, dev, N.stream_of(dev)),
             "aw4_route_forward")
-    return Routing(weights, chosen, totals[:experts], balance, logits, stats, totals, k, renormalize)
+    return Routing(weights, chosen, counts, balance, logits, stats, k, renormalize)
 
 
 def route_backward(dweights: torch.Tensor | None, dbalance: torch.Tensor | None,
@@ -110,7 +111,8 @@ def route_backward(dweights: torch.Tensor | None, dbalance: torch.Tensor | None,
     N.check(N.lib().aw4_route_backward(src.data_ptr(), N.DTYPE_CODES[logits.dtype], rows, experts, ld, routing.k,
                                        int(routing.renormalize), routing.weights.data_ptr(),
                                        routing.experts.data_ptr(), routing.stats.data_ptr(),
-                                       routing.totals.data_ptr(), N.ptr(dweights), N.ptr(dbalance),
+                                       routing.counts.data_ptr(), routing.stats.data_ptr() + 8 * rows,
+                                       N.ptr(dweights), N.ptr(dbalance),
                                        dlogits.data_ptr(), index, N.stream_of(index)), "aw4_route_backward")
     return dlogits
 
@@ -119,24 +121,23 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, valid, renormalize):
         r = route_forward(logits, k, valid, renormalize)
-        ctx.save_for_backward(r.weights, r.experts, logits, r.stats, r.totals)
+        ctx.save_for_backward(r.weights, r.experts, r.counts, logits, r.stats)
         ctx.k, ctx.renormalize = k, renormalize
-        ctx.mark_non_differentiable(r.experts, r.totals)
+        ctx.mark_non_differentiable(r.experts, r.counts)
         ctx.set_materialize_grads(False)
-        return r.weights, r.experts, r.totals, r.balance_loss
+        return r.weights, r.experts, r.counts, r.balance_loss
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dweights, _experts, _totals, dbalance):
-        weights, experts, logits, stats, totals = ctx.saved_tensors
-        r = Routing(weights, experts, totals[:-1], None, logits, stats, totals, ctx.k, ctx.renormalize)
+    def backward(ctx, dweights, _experts, _counts, dbalance):
+        weights, experts, counts, logits, stats = ctx.saved_tensors
+        r = Routing(weights, experts, counts, None, logits, stats, ctx.k, ctx.renormalize)
         return route_backward(dweights, dbalance, r), None, None, None
 
 
 def route(logits: torch.Tensor, k: int, valid: torch.Tensor | None = None, renormalize: bool = True) -> Routed:
     """Differentiable router; see the module's head."""
-    weights, experts, totals, balance = _Route.apply(logits, k, valid, renormalize)
-    return Routed(weights, experts, totals[:-1], balance)
+    return Routed(*_Route.apply(logits, k, valid, renormalize))
 
 
 def group_offsets(counts: torch.Tensor) -> torch.Tensor:

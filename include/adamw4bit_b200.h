@@ -269,22 +269,22 @@ int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, 
 /* ---------------------------------------------------------------------------
  * Expert router (no counterpart in the reference): softmax over the experts,
  * the k largest logits (ties to the lowest index; -inf never), their weights,
- * counts[experts] with the number of valid rows behind them (experts + 1
- * integers) and the balance loss sum_e (E counts_e / (k n)) mean(p_e).
+ * counts[experts], the number n of valid rows and the balance loss
+ * sum_e (E counts_e / (k n)) mean(p_e).
  * valid: NULL or one byte a row.  stats: two floats a row for the backward
- * call, 8-byte aligned.  Rows that are not valid, or all -inf: choices -1,
+ * call, 8-byte aligned; workspace 8-byte aligned, contents free.  Rows that are not valid, or all -inf: choices -1,
  * weights and gradients 0.  dweights and dbalance: NULL for zero.
  * ------------------------------------------------------------------------- */
 #define AW4_ROUTE_MAX_EXPERTS 1024
 uint64_t aw4_route_forward_workspace(int64_t rows, int32_t experts, int32_t device);
 int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
                           int32_t k, const uint8_t* valid, int32_t renormalize, float* weights,
-                          int32_t* chosen, float* stats, int32_t* counts, float* balance,
-                          void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+                          int32_t* chosen, float* stats, int32_t* counts, int32_t* valid_rows,
+                          float* balance, void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
 int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld,
                            int32_t k, int32_t renormalize, const float* weights, const int32_t* chosen,
-                           const float* stats, const int32_t* counts, const float* dweights,
-                           const float* dbalance, void* dlogits, int32_t device, void* stream);
+                           const float* stats, const int32_t* counts, const int32_t* valid_rows,
+                           const float* dweights, const float* dbalance, void* dlogits, int32_t device, void* stream);
 
 #ifdef __cplusplus
 }
