@@ -35,7 +35,7 @@ __device__ __forceinline__ int64_t warp_run(int run) {
     return ((int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5)) * run;
 }
 
-template <int DT>
+template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, uint8_t* __restrict__ codes,
                      uint8_t* __restrict__ scales) {
@@ -49,7 +49,7 @@ act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, u
     for (int j = 0; j < kChunks; ++j) {
         const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
         in[j] = c.in;
-        raw[j] = load_raw8<DT>(x, c.in ? c.row : 0, c.col, c.in ? cols : 0);
+        raw[j] = load_raw8<DT, WHOLE>(x, c.in ? c.row : 0, c.col, c.in ? cols : 0);
     }
     A8Block b[kChunks];
 #pragma unroll
@@ -63,7 +63,7 @@ act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, u
     store_scales(scales, unit0, units >> 2, b, lane);
 }
 
-template <int DT>
+template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
                        int cols, uint32_t per_row, const RowsOut out) {
@@ -87,7 +87,7 @@ act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restr
         if (!c.in) continue;
         float v[8];
         a8_decode8(q[j], a8_scale(b[j]), v);
-        store_raw8<DT>(out, c.row, c.col, cols, narrow8<DT>(v));
+        store_raw8<DT, WHOLE>(out, c.row, c.col, cols, narrow8<DT>(v));
     }
 }
 
@@ -113,7 +113,7 @@ __device__ __forceinline__ float sigmoid(float g) {
 // 167 with two, 205 with four).
 constexpr int kGluForward = 2, kGluBackward = 1;
 
-template <int DT, bool EMIT>
+template <int DT, bool WHOLE, bool EMIT>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols, uint32_t per_row,
                       const RowsOut h, uint8_t* __restrict__ gcodes, uint8_t* __restrict__ gscales,
@@ -128,8 +128,8 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
 #pragma unroll
     for (int j = 0; j < kGluForward; ++j) {
         at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
-        rg[j] = load_raw8<DT>(gate, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
-        ru[j] = load_raw8<DT>(up, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
+        rg[j] = load_raw8<DT, WHOLE>(gate, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
+        ru[j] = load_raw8<DT, WHOLE>(up, at[j].in ? at[j].row : 0, at[j].col, at[j].in ? cols : 0);
     }
 #pragma unroll
     for (int j = 0; j < kGluForward; ++j) {
@@ -154,7 +154,7 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
         if (!at[j].in) continue;
         *reinterpret_cast<uint2*>(gcodes + u * 8) = qg;
         *reinterpret_cast<uint2*>(ucodes + u * 8) = qu;
-        store_raw8<DT>(h, at[j].row, at[j].col, cols, r);
+        store_raw8<DT, WHOLE>(h, at[j].row, at[j].col, cols, r);
         if constexpr (EMIT) *reinterpret_cast<uint2*>(hcodes + u * 8) = qh;
         if ((lane & 3) == 0) {
             gscales[u >> 2] = (uint8_t)bg.byte;
@@ -165,7 +165,7 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
 }
 
 // dg = dh u (s + g s (1 - s)), du = dh g s, s = sigmoid(g)
-template <int DT>
+template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row,
                        const uint8_t* __restrict__ gcodes, const uint8_t* __restrict__ gscales,
@@ -184,7 +184,7 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
         const int64_t u = unit0 + j * 32 + lane;
         at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
         if (!at[j].in) continue;
-        rd[j] = load_raw8<DT>(dh, at[j].row, at[j].col, cols);
+        rd[j] = load_raw8<DT, WHOLE>(dh, at[j].row, at[j].col, cols);
         qg[j] = __ldcs(reinterpret_cast<const uint2*>(gcodes + u * 8));
         qu[j] = __ldcs(reinterpret_cast<const uint2*>(ucodes + u * 8));
         bg[j] = gscales[u >> 2];
@@ -208,8 +208,8 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
         vmul8(p, p, d);
         vmul8(p, p, s);
         vmul8(g, g, d);
-        store_raw8<DT>(dgate, at[j].row, at[j].col, cols, narrow8<DT>(p));
-        store_raw8<DT>(dup, at[j].row, at[j].col, cols, narrow8<DT>(g));
+        store_raw8<DT, WHOLE>(dgate, at[j].row, at[j].col, cols, narrow8<DT>(p));
+        store_raw8<DT, WHOLE>(dup, at[j].row, at[j].col, cols, narrow8<DT>(g));
     }
 }
 
@@ -300,7 +300,7 @@ constexpr int norm_blocks(int threads) {
 // 96 at 768 and 105 at 1024, where its sums spill).
 constexpr int kNormForward = 1024, kNormBackward = 512;
 
-template <int DT, int NT, int V>
+template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
 rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, int per_row,
                         const void* __restrict__ w, int w_dtype, float eps, const RowsOut y,
@@ -316,13 +316,13 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, 
     Raw8<DT> raw[V];
     if (row < rows)
 #pragma unroll
-        for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT>(x, row, (j * NT + t) * 8, cols);
+        for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT, WHOLE>(x, row, (j * NT + t) * 8, cols);
     stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
     for (int slot = 0; row < rows; row += step, slot ^= 1) {
         Raw8<DT> next[V];
         if (row + step < rows)
 #pragma unroll
-            for (int j = 0; j < V; ++j) next[j] = load_raw8<DT>(x, row + step, (j * NT + t) * 8, cols);
+            for (int j = 0; j < V; ++j) next[j] = load_raw8<DT, WHOLE>(x, row + step, (j * NT + t) * 8, cols);
         f2 ss = pk2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -358,7 +358,7 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, 
             if (u < per_row) {
                 *reinterpret_cast<uint2*>(code_row + u * 8) = q;
                 if ((t & 3) == 0) scale_row[u >> 2] = (uint8_t)b.byte;
-                store_raw8<DT>(y, row, u * 8, cols, ry);
+                store_raw8<DT, WHOLE>(y, row, u * 8, cols, ry);
                 if (ycodes) {
                     *reinterpret_cast<uint2*>(ycodes + row * per_row * 8 + u * 8) = qy;
                     if ((t & 3) == 0) yscales[(row * per_row + u) >> 2] = (uint8_t)by.byte;
@@ -379,7 +379,7 @@ struct NormRow {
     float r;
 };
 
-template <int DT, int NT, int V>
+template <int DT, int NT, int V, bool WHOLE>
 __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& dy, int64_t row, int t, int cols,
                                               int per_row, const uint8_t* codes, const uint8_t* scales,
                                               const float* rstd) {
@@ -388,7 +388,7 @@ __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& d
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int u = j * NT + t;
-        n.dy[j] = load_raw8<DT>(dy, row, u * 8, cols);
+        n.dy[j] = load_raw8<DT, WHOLE>(dy, row, u * 8, cols);
         n.q[j] = make_uint2(0, 0);
         n.b[j] = 1;
         if (u < per_row) {
@@ -401,7 +401,7 @@ __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& d
 
 // dx = r (w dy) - v r^3 mean(v w dy); each block leaves its rows' sum of
 // dy v r in partial[blockIdx.x][cols].
-template <int DT, int NT, int V>
+template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormBackward))
 rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols, int per_row,
                          const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
@@ -420,12 +420,12 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
     NormRow<DT, V> now;
-    if (row < rows) load_norm_row<DT, NT, V>(now, dy, row, t, cols, per_row, codes, scales, rstd);
+    if (row < rows) load_norm_row<DT, NT, V, WHOLE>(now, dy, row, t, cols, per_row, codes, scales, rstd);
     stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
     for (int slot = 0; row < rows; row += step, slot ^= 1) {
         NormRow<DT, V> next;
         if (row + step < rows)
-            load_norm_row<DT, NT, V>(next, dy, row + step, t, cols, per_row, codes, scales, rstd);
+            load_norm_row<DT, NT, V, WHOLE>(next, dy, row + step, t, cols, per_row, codes, scales, rstd);
         const float r = now.r;
         f2 dot2 = pk2(0.0f, 0.0f);
 #pragma unroll
@@ -435,7 +435,7 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
             a8_decode8(now.q[j], a8_scale(now.b[j]), v);
             vmul8(d, d, v);
             // behind the last column codes and gradients are zero, but a block may be NaN
-            if ((j * NT + t) * 8 + 8 > cols)
+            if (!WHOLE && (j * NT + t) * 8 + 8 > cols)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if ((j * NT + t) * 8 + i >= cols) d[i] = 0.0f;
@@ -457,7 +457,7 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
             vmul8(d, d, wv);
             vmuls8(d, d, r);
             vfmas8(d, -k, v, d);
-            if (u < per_row) store_raw8<DT>(dx, row, u * 8, cols, narrow8<DT>(d));
+            if (u < per_row) store_raw8<DT, WHOLE>(dx, row, u * 8, cols, narrow8<DT>(d));
         }
         now = next;
     }
@@ -564,6 +564,12 @@ static int32_t by_dtype(int dtype, F f) {
     return f(std::integral_constant<int, AW4_F16>());
 }
 
+// f(dtype, whether all of the call's rows are whole vectors)
+template <typename F>
+static int32_t by_form(int dtype, bool whole, F f) {
+    return by_dtype(dtype, [&](auto dt) { return whole ? f(dt, std::true_type()) : f(dt, std::false_type()); });
+}
+
 constexpr int64_t kNormCols = 16384;
 
 // Where a warp has a row: warps of a block, one for each SM's share of few rows.
@@ -603,9 +609,11 @@ extern "C" int32_t aw4_act8_quantize(const void* x, int32_t dtype, int64_t rows,
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
-    return by_dtype(dtype, [&](auto dt) {
-        act8_quantize_kernel<dt.value><<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(
-            rows_in(x, rows, cols, ld, dtype), rows, (int)cols, per_row, codes, scales);
+    const RowsIn in = rows_in(x, rows, cols, ld, dtype);
+    return by_form(dtype, in.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+        act8_quantize_kernel<dt.value, whole.value>
+            <<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(in, rows, (int)cols, per_row,
+                                                                                     codes, scales);
         return launched("act8_quantize");
     });
 }
@@ -620,9 +628,11 @@ extern "C" int32_t aw4_act8_dequantize(const uint8_t* codes, const uint8_t* scal
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
-    return by_dtype(dtype, [&](auto dt) {
-        act8_dequantize_kernel<dt.value><<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(
-            codes, scales, rows, (int)cols, per_row, rows_out(out, ld, dtype));
+    const RowsOut to = rows_out(out, ld, dtype);
+    return by_form(dtype, to.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+        act8_dequantize_kernel<dt.value, whole.value>
+            <<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(codes, scales, rows, (int)cols,
+                                                                                     per_row, to);
         return launched("act8_dequantize");
     });
 }
@@ -642,12 +652,12 @@ extern "C" int32_t aw4_swiglu_forward(const void* gate, const void* up, int32_t 
     const RowsIn g = rows_in(gate, rows, cols, ld_gate, dtype), u = rows_in(up, rows, cols, ld_up, dtype);
     const RowsOut o = rows_out(h, cols, dtype);
     const unsigned grid = run_grid(rows * per_row, 32 * kGluForward);
-    return by_dtype(dtype, [&](auto dt) {
+    return by_form(dtype, g.vec && u.vec && o.vec && cols % 8 == 0, [&](auto dt, auto whole) {
         if (hcodes)
-            swiglu_forward_kernel<dt.value, true><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
+            swiglu_forward_kernel<dt.value, whole.value, true><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
                 g, u, rows, (int)cols, per_row, o, gcodes, gscales, ucodes, uscales, hcodes, hscales);
         else
-            swiglu_forward_kernel<dt.value, false><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
+            swiglu_forward_kernel<dt.value, whole.value, false><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
                 g, u, rows, (int)cols, per_row, o, gcodes, gscales, ucodes, uscales, nullptr, nullptr);
         return launched("swiglu_forward");
     });
@@ -665,11 +675,12 @@ extern "C" int32_t aw4_swiglu_backward(const void* dh, int32_t dtype, int64_t ro
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
-    return by_dtype(dtype, [&](auto dt) {
-        swiglu_backward_kernel<dt.value>
+    const RowsIn in = rows_in(dh, rows, cols, ld_dh, dtype);
+    const RowsOut dg = rows_out(dgate, ld_out, dtype), du = rows_out(dup, ld_out, dtype);
+    return by_form(dtype, in.vec && dg.vec && du.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+        swiglu_backward_kernel<dt.value, whole.value>
             <<<run_grid(rows * per_row, 32 * kGluBackward), kA8Threads, 0, (cudaStream_t)stream>>>(
-                rows_in(dh, rows, cols, ld_dh, dtype), rows, (int)cols, per_row, gcodes, gscales, ucodes, uscales,
-                rows_out(dgate, ld_out, dtype), rows_out(dup, ld_out, dtype));
+                in, rows, (int)cols, per_row, gcodes, gscales, ucodes, uscales, dg, du);
         return launched("swiglu_backward");
     });
 }
@@ -690,15 +701,16 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
     DeviceGuard guard(device);
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
-    return by_dtype(dtype, [&](auto dt) {
+    const RowsIn in = rows_in(x, rows, cols, ld, dtype);
+    const RowsOut out = rows_out(y, cols, dtype);
+    return by_form(dtype, in.vec && out.vec && cols % 8 == 0, [&](auto dt, auto whole) {
         return norm_shape(cols, [&](auto nt, auto v) {
-            auto kernel = rms_norm_forward_kernel<dt.value, nt.value, v.value>;
+            auto kernel = rms_norm_forward_kernel<dt.value, nt.value, v.value, whole.value>;
             const int bytes = nt.value * v.value * 32;
             if (const int32_t rc = norm_smem(kernel, bytes)) return rc;
             kernel<<<norm_grid<nt.value>(device, rows, kNormForward), norm_threads<nt.value>(device, rows), bytes,
-                     (cudaStream_t)stream>>>(rows_in(x, rows, cols, ld, dtype), rows, (int)cols, 1.0f / (float)cols,
-                                             (int)per_row, weight, weight_dtype, eps, rows_out(y, cols, dtype), rstd,
-                                             codes, scales, ycodes, yscales);
+                     (cudaStream_t)stream>>>(in, rows, (int)cols, 1.0f / (float)cols, (int)per_row, weight,
+                                             weight_dtype, eps, out, rstd, codes, scales, ycodes, yscales);
             return launched("rms_norm_forward");
         });
     });
@@ -741,15 +753,17 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
                     (long long)workspace_bytes);
     const uint32_t per_row = chunks_per_row(cols);
     int grid = 0;
-    const int32_t rc = by_dtype(dtype, [&](auto dt) {
+    const RowsIn in = rows_in(dy, rows, cols, ld, dtype);
+    const RowsOut out = rows_out(dx, cols, dtype);
+    const int32_t rc = by_form(dtype, in.vec && out.vec && cols % 8 == 0, [&](auto dt, auto whole) {
         return norm_shape(cols, [&](auto nt, auto v) {
-            auto kernel = rms_norm_backward_kernel<dt.value, nt.value, v.value>;
+            auto kernel = rms_norm_backward_kernel<dt.value, nt.value, v.value, whole.value>;
             const int bytes = nt.value * v.value * 32;
             if (const int32_t rc = norm_smem(kernel, bytes)) return rc;
             grid = norm_grid<nt.value>(device, rows, kNormBackward);
             kernel<<<grid, norm_threads<nt.value>(device, rows), bytes, s>>>(
-                rows_in(dy, rows, cols, ld, dtype), rows, (int)cols, 1.0f / (float)cols, (int)per_row, codes, scales,
-                rstd, weight, weight_dtype, rows_out(dx, cols, dtype), workspace);
+                in, rows, (int)cols, 1.0f / (float)cols, (int)per_row, codes, scales, rstd, weight, weight_dtype,
+                out, workspace);
             return launched("rms_norm_backward");
         });
     });

@@ -35,7 +35,10 @@ struct Raw8 {
     uint4 w[Elem<DT>::kBytes / 2];
 };
 
-// Rows of a matrix in memory.  `vec`: every row starts on 16 bytes.
+// Rows of a matrix in memory.  `vec`: every row starts on 16 bytes.  Kernels come in two
+// forms: WHOLE where that holds for all their matrices and rows are whole chunks of eight, so that
+// every access is one of vectors and the code for the others is not in the way (router backward:
+// 400 instructions a row without).
 struct RowsIn {
     const char* base;
     const char* end;      // behind the last value
@@ -48,13 +51,18 @@ struct RowsOut {
     bool vec;
 };
 
-// Values [col, col + 8) of a row; zeros from `cols` on.
-template <int DT>
-__device__ __forceinline__ Raw8<DT> load_raw8(const RowsIn& m, int64_t row, int col, int cols) {
+// Values [col, col + 8) of the row that has its column `col` at p; zeros from `cols` on.
+template <int DT, bool WHOLE>
+__device__ __forceinline__ Raw8<DT> load_raw8_at(const RowsIn& m, const char* p, int col, int cols) {
     constexpr int kSize = Elem<DT>::kBytes, kWords = kSize * 2;
     Raw8<DT> r;
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int i = 0; i < kSize / 2; ++i)
+            r.w[i] = col < cols ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        return r;
+    }
     uint32_t* w = reinterpret_cast<uint32_t*>(r.w);
-    const char* p = m.base + (row * m.ld + col) * kSize;
     if (col + 8 <= cols) {
         if (m.vec) {
 #pragma unroll
@@ -96,11 +104,21 @@ __device__ __forceinline__ Raw8<DT> load_raw8(const RowsIn& m, int64_t row, int 
     return r;
 }
 
-template <int DT>
-__device__ __forceinline__ void store_raw8(const RowsOut& m, int64_t row, int col, int cols, const Raw8<DT>& r) {
+template <int DT, bool WHOLE>
+__device__ __forceinline__ Raw8<DT> load_raw8(const RowsIn& m, int64_t row, int col, int cols) {
+    return load_raw8_at<DT, WHOLE>(m, m.base + (row * m.ld + col) * Elem<DT>::kBytes, col, cols);
+}
+
+template <int DT, bool WHOLE>
+__device__ __forceinline__ void store_raw8_at(const RowsOut& m, char* p, int col, int cols, const Raw8<DT>& r) {
     constexpr int kSize = Elem<DT>::kBytes;
+    if constexpr (WHOLE) {
+        if (col < cols)
+#pragma unroll
+            for (int i = 0; i < kSize / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+        return;
+    }
     const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
-    char* p = m.base + (row * m.ld + col) * kSize;
     if (col + 8 <= cols) {
         if (m.vec) {
 #pragma unroll
@@ -189,6 +207,11 @@ __device__ __forceinline__ Raw8<DT> narrow8(const float v[8]) {
         }
     }
     return r;
+}
+
+template <int DT, bool WHOLE>
+__device__ __forceinline__ void store_raw8(const RowsOut& m, int64_t row, int col, int cols, const Raw8<DT>& r) {
+    store_raw8_at<DT, WHOLE>(m, m.base + (row * m.ld + col) * Elem<DT>::kBytes, col, cols, r);
 }
 
 // Larger magnitude of two words' values (its sign is not meaningful); a NaN is above every number.

@@ -71,7 +71,8 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 template <int DT, int L, int V, bool kPacked = DT != AW4_F32>
 struct Picker {
     uint32_t key[V];
-    __device__ __forceinline__ Picker(const float l[V], int) {
+    static constexpr int kShared = 0;      // words of shared memory a thread
+    __device__ __forceinline__ Picker(const float l[V], int, uint32_t*, int) {
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = order_key(l[i]);
     }
@@ -110,12 +111,18 @@ struct Picker {
 
 // 16-bit logits: their order in the upper half of a word and the index, counted
 // down, in the lower.  Words are then all different and one maximum gives both.
-// Eight of a lane are sorted once (Batcher's odd-even merge); a lane's largest is then its first.
+// Eight of a lane are sorted once (Batcher's odd-even merge) and wait in shared memory; a
+// lane holds its largest, and the lane that had the row's takes its next.
 template <int DT, int L, int V>
 struct Picker<DT, L, V, true> {
+    static constexpr int kShared = V == 8 ? 8 : 0;
     uint32_t key[V];
+    uint32_t* rest;      // the next of this lane's keys
+    int stride;
 
-    __device__ __forceinline__ Picker(const float l[V], int lane) {
+    __device__ __forceinline__ Picker(const float l[V], int lane, uint32_t* shared, int threads) {
+        rest = shared + threadIdx.x;
+        stride = threads;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int e = expert_of<L>(lane, i);
@@ -135,6 +142,9 @@ struct Picker<DT, L, V, true> {
                 key[kA[c]] = max(a, b);
                 key[kB[c]] = min(a, b);
             }
+#pragma unroll
+            for (int i = 1; i < V; ++i) rest[(i - 1) * stride] = key[i];
+            rest[(V - 1) * stride] = 0;
         }
     }
     __device__ __forceinline__ uint32_t next(int, int&) {
@@ -144,9 +154,10 @@ struct Picker<DT, L, V, true> {
             for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
         const uint32_t best = lanes_max<L>(mine);
         if constexpr (V == 8) {
-            const bool won = key[0] == best;
-#pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = won ? (i + 1 < V ? key[i + 1] : 0u) : key[i];
+            if (mine == best && best) {
+                key[0] = *rest;
+                rest += stride;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -166,18 +177,25 @@ struct Picker<DT, L, V, true> {
     }
 };
 
-// A row's logits, -inf in the place of those that take no part.
-template <int DT, int L, int V>
-__device__ __forceinline__ void load_logits(const RowsIn& logits, int64_t row, int lane, int experts, bool in,
-                                            float l[V]) {
+// A row's logits as loaded, and widened with -inf in the place of those that take no part.  WHOLE: rows of
+// V L experts on 16 bytes.
+template <int DT, int L, int V, bool WHOLE>
+struct RowLogits {
+    Raw8<DT> raw[V / 8];
+    // p: where the row has the first of this lane's logits
+    __device__ __forceinline__ void load(const RowsIn& logits, const char* p, int lane, int experts, bool in) {
 #pragma unroll
-    for (int c = 0; c < V / 8; ++c)
-        widen8<DT>(load_raw8<DT>(logits, in ? row : 0, (c * L + lane) * 8, in ? experts : 0), l + c * 8);
-    if (!in || experts < L * V)
+        for (int c = 0; c < V / 8; ++c)
+            raw[c] = load_raw8_at<DT, WHOLE>(logits, p + c * L * 8 * Elem<DT>::kBytes, (c * L + lane) * 8, in ? experts : 0);
+    }
+    __device__ __forceinline__ void widen(float l[V], int lane, int experts, bool in) const {
+#pragma unroll
+        for (int c = 0; c < V / 8; ++c) widen8<DT>(raw[c], l + c * 8);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (!in || expert_of<L>(lane, i) >= experts) l[i] = -INFINITY;
-}
+            if (!in || (!WHOLE && expert_of<L>(lane, i) >= experts)) l[i] = -INFINITY;
+    }
+};
 
 // Threads of a forward block: a block an SM, its sums over rows in registers.
 template <int V>
@@ -197,7 +215,7 @@ __host__ __device__ constexpr int64_t route_totals_bytes(int experts) {
     return (int64_t)sizeof(RouteTotals) + 12 * (int64_t)experts;
 }
 
-template <int DT, int L, int V>
+template <int DT, int L, int V, bool WHOLE>
 __global__ void __launch_bounds__(kRouteThreads<V>, 1)
 route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, const uint8_t* __restrict__ valid,
                      bool renormalize, float* __restrict__ weights, int32_t* __restrict__ chosen,
@@ -215,18 +233,31 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
     uint32_t* my_key = key_s + group * k;
     int32_t* my_chosen = chosen_s + group * k;
+    uint32_t* sorted_s = reinterpret_cast<uint32_t*>(chosen_s + kRows * k);   // what a Picker keeps
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    const int64_t tiles = (rows + kRows - 1) / kRows;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t row = tile * kRows + group;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + group;
+    // the next row's logits are on their way while one is worked on
+    RowLogits<DT, L, V, WHOLE> now;
+    uint8_t now_valid = 1;
+    const char* from = logits.base + (row * logits.ld + lane * 8) * Elem<DT>::kBytes;
+    const int64_t from_step = step * logits.ld * Elem<DT>::kBytes, k_step = step * k;
+    now.load(logits, from, lane, experts, row < rows);
+    if (valid && row < rows) now_valid = valid[row];
+    int64_t picks_at = row * k;
+    for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows;
+         base += step, row += step, picks_at += k_step) {
         const bool in = row < rows;
-        bool ok = in && (!valid || valid[row]);
+        bool ok = in && now_valid;
         float l[V];
-        load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
+        now.widen(l, lane, experts, ok);
+        from += from_step;
+        now.load(logits, from, lane, experts, row + step < rows);
+        if (valid && row + step < rows) now_valid = valid[row + step];
         using P = Picker<DT, L, V>;
-        P picker(l, lane);
+        P picker(l, lane, sorted_s, kThreads);
         // the k largest, kept by the lanes in turn
         int at = 0;
         const uint32_t first = picker.next(lane, at);
@@ -271,8 +302,8 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
             for (int j = lane; j < k; j += L) {       // its own choices
                 const bool take = ok && P::some(my_key[j]);
                 const int e = take ? P::expert(my_key[j], DT == AW4_F32 ? my_chosen[j] : 0) : -1;
-                weights[row * k + j] = take ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
-                chosen[row * k + j] = e;
+                weights[picks_at + j] = take ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
+                chosen[picks_at + j] = e;
                 if (take) atomicAdd(&count[e], 1);
             }
         }
@@ -336,9 +367,11 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
 }
 
 constexpr int kRouteBackThreads = 256;
+template <int V>
+constexpr int kRouteBackBlocks = V == 8 ? 4 : 2;        // resident on an SM
 
-template <int DT, int L, int V>
-__global__ void __launch_bounds__(kRouteBackThreads)
+template <int DT, int L, int V, bool WHOLE>
+__global__ void __launch_bounds__(kRouteBackThreads, kRouteBackBlocks<V>)
 route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, bool renormalize,
                       const float* __restrict__ weights, const int32_t* __restrict__ chosen,
                       const float2* __restrict__ stats, const int32_t* __restrict__ counts,
@@ -360,38 +393,59 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         const int e = expert_of<L>(lane, i);
         share[i] = e < experts ? (float)counts[e] * unit : 0.0f;
     }
-    const int64_t tiles = (rows + kRows - 1) / kRows;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t row = tile * kRows + group;
-        const bool in = row < rows;
-        const float2 st = in ? stats[row] : make_float2(0.0f, 0.0f);
-        const bool ok = st.y != 0.0f;             // a NaN row is a valid one
-        // a lane's first choice is loaded with the logits
-        const int picks = dweights && in ? k : 0;
-        int at = -1;
-        float w = 0.0f, d = 0.0f;
-        if (lane < picks) {
-            at = chosen[row * k + lane];
-            w = weights[row * k + lane];
-            d = dweights[row * k + lane];
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + group;
+    // The next row is on its way while one is worked on: its logits, its statistics and a
+    // lane's first choice.
+    RowLogits<DT, L, V, WHOLE> now;
+    float2 now_st;
+    int now_at;
+    float now_w, now_d;
+    const char* from = logits.base + (row * logits.ld + lane * 8) * Elem<DT>::kBytes;
+    const int64_t from_step = step * logits.ld * Elem<DT>::kBytes, k_step = step * k;
+    char* to = dlogits.base + (row * experts + lane * 8) * Elem<DT>::kBytes;
+    const int64_t to_step = step * experts * Elem<DT>::kBytes;
+    int64_t picks_at = row * k;
+    auto fetch = [&](int64_t r, int64_t picks_r) {
+        const bool in = r < rows;
+        now.load(logits, from, lane, experts, in);
+        now_st = in ? stats[r] : make_float2(0.0f, 0.0f);
+        now_at = -1;
+        now_w = now_d = 0.0f;
+        if (in && dweights && lane < k) {
+            now_at = chosen[picks_r + lane];
+            now_w = weights[picks_r + lane];
+            now_d = dweights[picks_r + lane];
         }
+    };
+    fetch(row, picks_at);
+    for (int64_t base = (int64_t)blockIdx.x * kRows; base < rows;
+         base += step, row += step, picks_at += k_step, to += to_step) {
+        const bool in = row < rows;
+        const float2 st = now_st;
+        const bool ok = st.y != 0.0f;             // a NaN row is a valid one
+        const int picks = dweights && in ? k : 0;
+        int at = now_at;
+        float w = now_w, d = now_d;
         float l[V];
-        load_logits<DT, L, V>(logits, row, lane, experts, ok, l);
+        now.widen(l, lane, experts, ok);
+        from += from_step;
+        fetch(row + step, picks_at + k_step);
         float inner = 0.0f;
         for (int j = lane; j < picks; j += L) {
             if (j != lane) {
-                at = chosen[row * k + j];
-                w = weights[row * k + j];
-                d = dweights[row * k + j];
+                at = chosen[picks_at + j];
+                w = weights[picks_at + j];
+                d = dweights[picks_at + j];
             }
             if (at >= 0) inner = __fmaf_rn(w, d, inner);
         }
         inner = lanes_sum<L>(inner);
         for (int j = lane; j < picks; j += L) {
             if (k > L) {
-                at = chosen[row * k + j];
-                w = weights[row * k + j];
-                d = dweights[row * k + j];
+                at = chosen[picks_at + j];
+                w = weights[picks_at + j];
+                d = dweights[picks_at + j];
             }
             if (at >= 0) mine[at] = w * (d - (renormalize ? inner : 0.0f));
         }
@@ -408,13 +462,14 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         for (int i = 0; i < V; ++i) l[i] = __fmaf_rn(l[i], share[i] - off, mine[expert_of<L>(lane, i)]);
         __syncwarp();
         for (int j = lane; j < picks; j += L) {
-            if (k > L) at = chosen[row * k + j];
+            if (k > L) at = chosen[picks_at + j];
             if (at >= 0) mine[at] = 0.0f;
         }
         if (in)
 #pragma unroll
             for (int c = 0; c < V / 8; ++c)
-                store_raw8<DT>(dlogits, row, (c * L + lane) * 8, experts, narrow8<DT>(l + c * 8));
+                store_raw8_at<DT, WHOLE>(dlogits, to + c * L * 8 * Elem<DT>::kBytes, (c * L + lane) * 8, experts,
+                                  narrow8<DT>(l + c * 8));
         __syncwarp();
     }
 }
@@ -439,6 +494,14 @@ static int32_t route_by_dtype(int dtype, F f) {
     if (dtype == AW4_F32) return f(integral_constant<int, AW4_F32>());
     if (dtype == AW4_BF16) return f(integral_constant<int, AW4_BF16>());
     return f(integral_constant<int, AW4_F16>());
+}
+
+// The form of a call: WHOLE only up to 256 experts, eight logits a lane.
+template <int V, typename F>
+static int32_t route_form(bool whole, F f) {
+    if constexpr (V == 8)
+        if (whole) return f(std::true_type());
+    return f(std::false_type());
 }
 
 static int32_t check_route(const char* what, int dtype, int64_t rows, int64_t experts, int32_t k) {
@@ -513,20 +576,25 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
         return route_shape(experts, [&](auto lanes, auto v) {
             constexpr int kThreads = kRouteThreads<v.value>;
             // choices of the rows in work, later the warps' sums
-            const int choices = std::max(2 * (kThreads / lanes.value) * k, kThreads / 32 * v.value * lanes.value);
-            auto kernel = route_forward_kernel<dt.value, lanes.value, v.value>;
+            const int choices = std::max(2 * (kThreads / lanes.value) * k +
+                                             Picker<dt.value, lanes.value, v.value>::kShared * kThreads,
+                                         kThreads / 32 * v.value * lanes.value);
+            const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
+            return route_form<v.value>(in.vec && experts == lanes.value * v.value, [&](auto whole) {
+            auto kernel = route_forward_kernel<dt.value, lanes.value, v.value, whole.value>;
             const int bytes = (experts + 1 + choices) * 4;
             if (bytes > 40 * 1024) {
                 const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
                 if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
             }
-            kernel<<<grid, kThreads, bytes, s>>>(route_rows(logits, rows, experts, ld, dtype), rows, experts, k, valid,
+            kernel<<<grid, kThreads, bytes, s>>>(in, rows, experts, k, valid,
                                                  renormalize != 0, weights, chosen, reinterpret_cast<float2*>(stats),
                                                  static_cast<RouteTotals*>(workspace), counts, valid_rows, balance);
             note_launch();
             const cudaError_t e = cudaGetLastError();
             return e == cudaSuccess ? (int32_t)AW4_OK
                                     : fail(AW4_ERR_CUDA, "route_forward launch: %s", cudaGetErrorString(e));
+            });
         });
     });
 }
@@ -545,16 +613,20 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
     return route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
             const int per = kRouteBackThreads / lanes.value;
-            const int grid = (int)std::min<int64_t>((rows + per - 1) / per, (int64_t)sm_count(device) * 8);
-            route_backward_kernel<dt.value, lanes.value, v.value>
+            const int grid = (int)std::min<int64_t>((rows + per - 1) / per,
+                                                   (int64_t)sm_count(device) * kRouteBackBlocks<v.value>);
+            const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
+            const RowsOut out = {static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)};
+            return route_form<v.value>(in.vec && out.vec && experts == lanes.value * v.value, [&](auto whole) {
+            route_backward_kernel<dt.value, lanes.value, v.value, whole.value>
                 <<<grid, kRouteBackThreads, 0, (cudaStream_t)stream>>>(
-                    route_rows(logits, rows, experts, ld, dtype), rows, experts, k, renormalize != 0, weights, chosen,
-                    reinterpret_cast<const float2*>(stats), counts, valid_rows, dweights, dbalance,
-                    RowsOut{static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)});
+                    in, rows, experts, k, renormalize != 0, weights, chosen, reinterpret_cast<const float2*>(stats),
+                    counts, valid_rows, dweights, dbalance, out);
             note_launch();
             const cudaError_t e = cudaGetLastError();
-            return e == cudaSuccess ? AW4_OK
+            return e == cudaSuccess ? (int32_t)AW4_OK
                                     : fail(AW4_ERR_CUDA, "route_backward launch: %s", cudaGetErrorString(e));
+            });
         });
     });
 }

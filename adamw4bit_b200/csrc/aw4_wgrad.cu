@@ -617,11 +617,11 @@ weight_grad_join_kernel(const WgParams p, int pairs) {
         for (int i = 0; i < 8; ++i) f[i] = tile[r][lane * 8 + i];
         if (p.accumulate) {
             float o[8];
-            widen8<OT>(load_raw8<OT>(old, row, at, p.k), o);
+            widen8<OT>(load_raw8<OT, false>(old, row, at, p.k), o);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] += o[i];
         }
-        store_raw8<OT>(out, row, at, p.k, narrow8<OT>(f));
+        store_raw8<OT, false>(out, row, at, p.k, narrow8<OT>(f));
     }
 }
 
