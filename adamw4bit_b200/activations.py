@@ -45,14 +45,14 @@ BLOCK = 32
 
 
 class Act8:
-    """The 8-bit checkpoint of a tensor: its codes and block exponents in one buffer (``data``), and the
-    shape and dtype it reads back as.  ``codes`` is int8 [rows, cols rounded up to 32], ``scales`` uint8
+    """The 8-bit checkpoint of a tensor: its codes and block exponents in a buffer (``data``, from byte
+    ``start`` on), and the shape and dtype it reads back as.  ``codes`` is int8 [rows, cols rounded up to 32], ``scales`` uint8
     [rows, blocks] with e + 127 (255: the block was not finite)."""
 
-    __slots__ = ("data", "shape", "dtype", "rows", "cols")
+    __slots__ = ("data", "shape", "dtype", "rows", "cols", "start")
 
-    def __init__(self, data: torch.Tensor, shape, dtype: torch.dtype):
-        self.data, self.shape, self.dtype = data, shape, dtype
+    def __init__(self, data: torch.Tensor, shape, dtype: torch.dtype, start: int = 0):
+        self.data, self.shape, self.dtype, self.start = data, shape, dtype, start
         self.cols = shape[-1]
         self.rows = math.prod(shape[:-1])
 
@@ -62,17 +62,17 @@ class Act8:
 
     @property
     def nbytes(self) -> int:
-        return self.data.numel()
+        return self.rows * -(-self.cols // BLOCK) * (BLOCK + 1)
 
     @property
     def codes(self) -> torch.Tensor:
-        blocks = -(-self.cols // BLOCK)
-        return self.data[: self.rows * blocks * BLOCK].view(torch.int8).view(self.rows, blocks * BLOCK)
+        pitch = -(-self.cols // BLOCK) * BLOCK
+        return self.data[self.start: self.start + self.rows * pitch].view(torch.int8).view(self.rows, pitch)
 
     @property
     def scales(self) -> torch.Tensor:
         blocks = -(-self.cols // BLOCK)
-        return self.data[self.rows * blocks * BLOCK:].view(self.rows, blocks)
+        return self.data[self.start + self.rows * blocks * BLOCK: self.start + self.nbytes].view(self.rows, blocks)
 
     def dequantize(self) -> torch.Tensor:
         return dequantize_act8(self)
@@ -84,26 +84,42 @@ class Act8:
         return f"Act8(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
 
 
-def _empty_act8(t: torch.Tensor, shape, rows: int, cols: int) -> Act8:
-    """A checkpoint to be written for a tensor like t of this shape."""
+def _empty_act8(t: torch.Tensor, shape, rows: int, cols: int, more: int = 0) -> Act8:
+    """A checkpoint to be written for a tensor like t of this shape, and `more` bytes behind it."""
     x8 = Act8.__new__(Act8)
-    x8.data = t.new_empty(rows * (-(-cols // BLOCK)) * (BLOCK + 1), dtype=torch.uint8)
-    x8.shape, x8.dtype, x8.rows, x8.cols = shape, t.dtype, rows, cols
+    x8.data = t.new_empty(rows * (-(-cols // BLOCK)) * (BLOCK + 1) + more, dtype=torch.uint8)
+    x8.shape, x8.dtype, x8.rows, x8.cols, x8.start = shape, t.dtype, rows, cols, 0
     return x8
+
+
+def _second_act8(x8: Act8, start: int) -> Act8:
+    """Another checkpoint like x8 in the same buffer."""
+    y8 = Act8.__new__(Act8)
+    y8.data, y8.shape, y8.dtype, y8.rows, y8.cols, y8.start = x8.data, x8.shape, x8.dtype, x8.rows, x8.cols, start
+    return y8
 
 
 def _ptrs(x8: Act8) -> tuple[int, int]:
     """Addresses of codes and scales."""
-    p = x8.data.data_ptr()
+    p = x8.data.data_ptr() + x8.start
     return p, p + x8.rows * (-(-x8.cols // BLOCK)) * BLOCK
 
 
+def _second_start(rows: int, cols: int) -> int:
+    """Where a second checkpoint, or float32 statistics, begin behind a first: on 16 bytes."""
+    return -(-(rows * (-(-cols // BLOCK)) * (BLOCK + 1)) // 16) * 16
+
+
 class RMSNormSaved(NamedTuple):
-    """What ``rms_norm_forward`` keeps: the checkpoint of x and (mean(x^2) + eps)^-1/2 of its rows.
-    ``output`` is the checkpoint of y where it was asked for."""
+    """What ``rms_norm_forward`` keeps: the checkpoint of x, and behind it in the same buffer
+    (mean(x^2) + eps)^-1/2 of its rows.  ``output`` is the checkpoint of y where it was asked for."""
     x8: Act8
-    rstd: torch.Tensor
     output: Act8 | None = None
+
+    @property
+    def rstd(self) -> torch.Tensor:
+        start = _second_start(self.x8.rows, self.x8.cols)
+        return self.x8.data[start: start + 4 * self.x8.rows].view(torch.float32)
 
 
 class SwiGLUSaved(NamedTuple):
@@ -212,14 +228,14 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *
     weight = _check_weight(weight, cols, x.dtype, x.device, "rms_norm")
     dev = x.get_device()
     y = x.new_empty(x.shape)
-    rstd = x.new_empty(rows, dtype=torch.float32)
-    x8 = _empty_act8(x, x.shape, rows, cols)
+    start = _second_start(rows, cols)
+    x8 = _empty_act8(x, x.shape, rows, cols, start + 4 * rows - rows * (-(-cols // BLOCK)) * (BLOCK + 1))
     y8 = _empty_act8(x, x.shape, rows, cols) if checkpoint_output else None
     yc, ys = _ptrs(y8) if y8 is not None else (None, None)
     N.check(N.lib().aw4_rms_norm_forward(src.data_ptr(), code, rows, cols, ld, weight.data_ptr(),
-                                         N.DTYPE_CODES[weight.dtype], eps, y.data_ptr(), rstd.data_ptr(),
+                                         N.DTYPE_CODES[weight.dtype], eps, y.data_ptr(), x8.data.data_ptr() + start,
                                          *_ptrs(x8), yc, ys, dev, N.stream_of(dev)), "aw4_rms_norm_forward")
-    return y, RMSNormSaved(x8, rstd, y8)
+    return y, RMSNormSaved(x8, y8)
 
 
 def rms_norm_backward(dy: torch.Tensor, weight: torch.Tensor,
@@ -238,7 +254,7 @@ def rms_norm_backward(dy: torch.Tensor, weight: torch.Tensor,
     nbytes = _norm_workspace(rows, cols, dev)
     ws = dy.new_empty(nbytes, dtype=torch.uint8)
     N.check(N.lib().aw4_rms_norm_backward(src.data_ptr(), code, rows, cols, ld, *_ptrs(x8),
-                                          saved.rstd.data_ptr(), weight.data_ptr(),
+                                          x8.data.data_ptr() + _second_start(rows, cols), weight.data_ptr(),
                                           N.DTYPE_CODES[weight.dtype], dx.data_ptr(), dw.data_ptr(),
                                           ws.data_ptr(), nbytes, dev, N.stream_of(dev)), "aw4_rms_norm_backward")
     return dx, dw
@@ -248,7 +264,7 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, checkpoint_output):
         y, saved = rms_norm_forward(x, weight, eps, checkpoint_output=checkpoint_output)
-        ctx.save_for_backward(weight, saved.x8.data, saved.rstd)
+        ctx.save_for_backward(weight, saved.x8.data)
         ctx.x8 = (saved.x8.shape, saved.x8.dtype)
         y8 = saved.output.data if checkpoint_output else None
         if y8 is not None:
@@ -258,8 +274,8 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, _):
-        weight, data, rstd = ctx.saved_tensors
-        dx, dw = rms_norm_backward(dy, weight, RMSNormSaved(Act8(data, *ctx.x8), rstd))
+        weight, data = ctx.saved_tensors
+        dx, dw = rms_norm_backward(dy, weight, RMSNormSaved(Act8(data, *ctx.x8)))
         return dx, dw, None, None
 
 
@@ -296,7 +312,9 @@ def swiglu_forward(gate: torch.Tensor, up: torch.Tensor | None = None, *,
         other = up.data_ptr()
     dev = gate.get_device()
     h = gate.new_empty(shape)
-    g8, u8 = _empty_act8(gate, shape, rows, cols), _empty_act8(gate, shape, rows, cols)
+    start = _second_start(rows, cols)
+    g8 = _empty_act8(gate, shape, rows, cols, start)         # both in one buffer
+    u8 = _second_act8(g8, start)
     h8 = _empty_act8(gate, shape, rows, cols) if checkpoint_output else None
     hc, hs = _ptrs(h8) if h8 is not None else (None, None)
     N.check(N.lib().aw4_swiglu_forward(src.data_ptr(), other, code, rows, cols, ld, ld_up, h.data_ptr(),
@@ -330,8 +348,8 @@ class _SwiGLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, checkpoint_output):
         h, saved = swiglu_forward(gate, up, checkpoint_output=checkpoint_output)
-        ctx.save_for_backward(saved.gate8.data, saved.up8.data)
-        ctx.act8, ctx.packed = (saved.gate8.shape, saved.gate8.dtype), saved.packed
+        ctx.save_for_backward(saved.gate8.data)
+        ctx.act8, ctx.packed, ctx.start = (saved.gate8.shape, saved.gate8.dtype), saved.packed, saved.up8.start
         h8 = saved.output.data if checkpoint_output else None
         if h8 is not None:
             ctx.mark_non_differentiable(h8)
@@ -340,8 +358,9 @@ class _SwiGLU(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, _):
-        g, u = (Act8(d, *ctx.act8) for d in ctx.saved_tensors)
-        out = swiglu_backward(dh, SwiGLUSaved(g, u, ctx.packed))
+        data, = ctx.saved_tensors
+        saved = SwiGLUSaved(Act8(data, *ctx.act8), Act8(data, *ctx.act8, ctx.start), ctx.packed)
+        out = swiglu_backward(dh, saved)
         return (out, None, None) if ctx.packed else (*out, None)
 
 
@@ -423,11 +442,11 @@ def _check_linear(x: torch.Tensor, weight: torch.Tensor, x8: Act8 | None, what: 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, data):
-        if data is None and ctx.needs_input_grad[1]:
-            data = quantize_act8(x).data
-        ctx.save_for_backward(weight, data if ctx.needs_input_grad[1] else None)
-        ctx.x8 = (x.shape, x.dtype)
+    def forward(ctx, x, weight, bias, x8):
+        if x8 is None and ctx.needs_input_grad[1]:
+            x8 = quantize_act8(x)
+        ctx.save_for_backward(weight, x8.data if ctx.needs_input_grad[1] else None)
+        ctx.x8 = (x.shape, x.dtype, x8.start if x8 is not None else 0)
         return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
@@ -448,16 +467,17 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     _check_linear(x, weight, x8, "linear")
     if weight.dim() != 2:
         raise ValueError(f"linear: weight of two dimensions expected, found {tuple(weight.shape)}")
-    return _Linear.apply(x, weight, bias, None if x8 is None else x8.data)
+    return _Linear.apply(x, weight, bias, x8)
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, offsets, data):
-        if data is None and ctx.needs_input_grad[1]:
-            data = quantize_act8(x).data
-        ctx.save_for_backward(weight, offsets, data if ctx.needs_input_grad[1] else None)
-        ctx.x8, ctx.bounds = (x.shape, x.dtype), offsets.tolist()
+    def forward(ctx, x, weight, offsets, x8):
+        if x8 is None and ctx.needs_input_grad[1]:
+            x8 = quantize_act8(x)
+        ctx.save_for_backward(weight, offsets, x8.data if ctx.needs_input_grad[1] else None)
+        ctx.x8 = (x.shape, x.dtype, x8.start if x8 is not None else 0)
+        ctx.bounds = offsets.tolist()
         y = x.new_zeros(x.shape[0], weight.shape[1])
         for g, (a, b) in enumerate(zip(ctx.bounds, ctx.bounds[1:])):
             if b > a:
@@ -492,4 +512,4 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     _same(offsets, x.device, torch.int32, "grouped_linear: offsets")
     if offsets.shape != (weight.shape[0] + 1,):
         raise ValueError(f"grouped_linear: {weight.shape[0] + 1} offsets expected, found {tuple(offsets.shape)}")
-    return _GroupedLinear.apply(x, weight, offsets, None if x8 is None else x8.data)
+    return _GroupedLinear.apply(x, weight, offsets, x8)

@@ -298,14 +298,14 @@ __device__ __forceinline__ void wg_store(const WgParams& p, int64_t row_off, int
     if constexpr (!FROM32) {
         uint16_t* o = static_cast<uint16_t*>(p.out) + row_off + k;
         if (whole) {
-            __stcs(reinterpret_cast<uint4*>(o), w);
+            *reinterpret_cast<uint4*>(o) = w;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (k + i < p.k) o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
         }
     } else if (OT == AW4_F32 && whole && !p.accumulate) {
-        __stcs(reinterpret_cast<uint4*>(static_cast<uint32_t*>(p.out) + row_off + k), w);
+        *reinterpret_cast<uint4*>(static_cast<uint32_t*>(p.out) + row_off + k) = w;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -376,7 +376,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWgProduct) tmem_alloc(smem_addr(&s.tmem), 512);
-    wg_schedule(p, s, pair, pairs, side == 0);
+    wg_schedule(p, s, pair, pairs, side == 0 && p.slots);
     tc_fence_before();
     pair_sync();
     tc_fence_after();
@@ -673,7 +673,13 @@ static int wg_pairs(int device, int64_t rows, int64_t n, int64_t k, int64_t grou
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, sms / 2, kWgMaxPairs}));
 }
 
-static uint64_t wg_workspace(int pairs) {
+// One group's tiles, all of as many steps, in whole rounds of the pairs: none is cut.
+static bool wg_cuts(int pairs, int64_t n, int64_t k, int64_t groups) {
+    return groups > 1 || wg_tiles(n, k) % pairs != 0;
+}
+
+static uint64_t wg_workspace(int pairs, int64_t n, int64_t k, int64_t groups) {
+    if (!wg_cuts(pairs, n, k, groups)) return 0;
     return (uint64_t)pairs * 2 * (sizeof(WgSlot) + (uint64_t)kWgTileN * kWgTileK * sizeof(float));
 }
 
@@ -683,7 +689,7 @@ using namespace aw4;
 
 extern "C" uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device) {
     if (rows <= 0 || n <= 0 || k <= 0 || groups < 1) return 0;
-    return wg_workspace(wg_pairs(device, rows, n, k, groups));
+    return wg_workspace(wg_pairs(device, rows, n, k, groups), n, k, groups);
 }
 
 extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
@@ -714,7 +720,9 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     if (!dy || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)dy % 16 || ld < n || ld * 2 % 16)
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: null buffer, or rows not on 16 bytes");
     const int pairs = wg_pairs(device, rows, n, k, groups);
-    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)wg_workspace(pairs))
+    const bool cuts = wg_cuts(pairs, n, k, groups);
+    if (cuts && (!workspace || (uintptr_t)workspace % 16 ||
+                 workspace_bytes < (int64_t)wg_workspace(pairs, n, k, groups)))
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: workspace of %lld bytes is too small or misaligned",
                     (long long)workspace_bytes);
     if (!encode_tiled()) return fail(AW4_ERR_CUDA, "aw4_weight_grad: the driver has no cuTensorMapEncodeTiled");
@@ -732,7 +740,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     p.accumulate = accumulate != 0;
     p.vec_out = (uintptr_t)out % 16 == 0 && k * size % 16 == 0;
     p.partial = static_cast<float*>(workspace);
-    p.slots = reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK);
+    p.slots = cuts ? reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK) : nullptr;
     p.status = status;
     CUtensorMap dy_map, code_map;
     if (!encode_rows(&dy_map, dtype == AW4_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
@@ -748,9 +756,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
         note_launch();
         e = cudaGetLastError();
         if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "weight_grad launch: %s", cudaGetErrorString(e));
-        // without groups the host knows that pairs with whole tiles leave no parts
-        const int64_t tiles = (int64_t)p.n_tiles * p.k_tiles;
-        if (!offsets && tiles % pairs == 0) return AW4_OK;
+        if (!cuts) return AW4_OK;
         weight_grad_join_kernel<ot.value><<<dim3(pairs, kWgTileN / kWgSlice), 256, 0, s>>>(p, pairs);
         note_launch();
         e = cudaGetLastError();
