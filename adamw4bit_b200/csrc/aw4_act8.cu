@@ -487,21 +487,24 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
     }
 }
 
-// Column sums of partial[parts][cols], in a fixed order: 32 threads share a column.
+// Column sums of partial[parts][cols], in a fixed order: a block has eight columns (whole sectors), 32 threads
+// share a column.
+constexpr int kSumCols = 8;
+
 template <int DT>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(32 * kSumCols)
 column_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* __restrict__ out) {
-    __shared__ float s[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
+    __shared__ float s[kSumCols][33];
+    const int c = threadIdx.x % kSumCols, r = threadIdx.x / kSumCols, col = blockIdx.x * kSumCols + c;
     float v = 0.0f;
-    if (c < cols)
+    if (col < cols)
 #pragma unroll 8
-        for (int p = threadIdx.y; p < parts; p += 32) v += partial[(int64_t)p * cols + c];
-    s[threadIdx.y][threadIdx.x] = v;
+        for (int p = r; p < parts; p += 32) v += partial[(int64_t)p * cols + col];
+    s[c][r] = v;
     __syncthreads();
-    v = warp_sum(s[threadIdx.x][threadIdx.y]);
-    const int col = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && col < cols) Elem<DT>::store1(out, col, v);
+    const int mine = blockIdx.x * kSumCols + (threadIdx.x >> 5);
+    v = warp_sum(s[threadIdx.x >> 5][threadIdx.x & 31]);
+    if ((threadIdx.x & 31) == 0 && mine < cols) Elem<DT>::store1(out, mine, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -769,8 +772,8 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
     });
     if (rc) return rc;
     return by_dtype(weight_dtype, [&](auto wt) {
-        column_sum_kernel<wt.value><<<(int)((cols + 31) / 32), dim3(32, 32), 0, s>>>(workspace, grid, (int)cols,
-                                                                                    dweight);
+        column_sum_kernel<wt.value><<<(int)((cols + kSumCols - 1) / kSumCols), 32 * kSumCols, 0, s>>>(
+            workspace, grid, (int)cols, dweight);
         return launched("column_sum");
     });
 }
