@@ -296,9 +296,9 @@ template <int NT>
 constexpr int norm_blocks(int threads) {
     return NT == 32 ? threads / (32 * kNormWarps) : NT < threads ? threads / NT : 1;
 }
-// Forward: 1024 at 64 registers (56 us at 16384 x 4096 bf16; 58 at 768, 64 at 512).  Backward: 512 at 128 (70 us;
-// 96 at 768 and 105 at 1024, where its sums spill).
-constexpr int kNormForward = 1024, kNormBackward = 512;
+// Forward: 1024 at 64 registers (54 us at 16384 x 4096 bf16; 58 at 768, 64 at 512).  Backward: 768 at 85 (61 us;
+// 66 at 512, 103 at 1024, where its sums spill).
+constexpr int kNormForward = 1024, kNormBackward = 768;
 
 template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))

@@ -81,7 +81,7 @@ struct WgParams {
     void* out;
     bool accumulate, vec_out;
     float* partial;
-    WgSlot* slots;
+    WgSlot* slots;              // null: no tile is cut
     int32_t* status;
 };
 
@@ -132,12 +132,27 @@ __device__ __forceinline__ int64_t wg_block_sum(int64_t v, int64_t* part) {
     return v;
 }
 
+// Cutting evens the pairs' steps and costs the parts' way through memory and the second kernel, about as much
+// as this many steps: 4096 x 4096 x 4096, 128 tiles of 64 steps, takes 128 us cut over 74 pairs and 109 us as
+// two whole tiles on each of 64; 8192 x 14336 x 4096, 448 tiles of 128 steps, 690 us cut and 796 us in seven
+// rounds; 2048 x 768 x 768, 6 tiles of 32 steps, 30 us cut and 35 us whole.
+constexpr int kWgCutSteps = 24;
+
 // This pair's segments.  Tiles [cut, tiles) are laid end to end as row steps; a pair
-// takes as many as it lacks to the average of all pairs.  A thread looks at one pair, then at one cut tile.
-__device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs, bool writes) {
+// takes as many as it lacks to the average of all pairs.  A thread looks at one pair, then at one cut tile.  Where
+// whole tiles alone leave no pair more than kWgCutSteps above the average, none is cut.
+__device__ __noinline__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs, bool writes) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_group = p.n_tiles * p.k_tiles;
     const int tiles = per_group * p.groups;
+    if (tid == 0) {
+        s.whole = (tiles - pair + pairs - 1) / pairs;  // none is cut
+        s.cuts = 0;
+    }
+    if (!p.slots) {
+        __syncthreads();
+        return;
+    }
     const int whole = max(0, tiles / pairs - 1);       // whole tiles of every pair
     const int cut = whole * pairs;
     int64_t load = 0;
@@ -150,9 +165,12 @@ __device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs,
         }
     }
     const int steps = cut + tid < tiles ? wg_steps(p, (cut + tid) / per_group) : 0;
-    if (tid == 0) s.cuts = 0;
     const int64_t rest = wg_block_sum(steps, s.part[0]);
     const int64_t target = (wg_block_sum(load, s.part[1]) + rest + pairs - 1) / pairs;
+    if (writes && tid < 2) p.slots[2 * pair + tid] = {-1, 0};
+    int64_t uncut = load;
+    for (int t = cut + tid; tid < pairs && t < tiles; t += pairs) uncut += wg_steps(p, t / per_group);
+    if (!wg_block_sum(tid < pairs && uncut - target > kWgCutSteps, s.part[0])) return;
     const int64_t lack = tid < pairs ? max((int64_t)0, target - load) : 0;
     const int64_t from = min(rest, wg_block_sum(tid < pair ? lack : 0, s.part[0]));
     const int64_t to = min(rest, from + wg_block_sum(tid == pair ? lack : 0, s.part[1]));
@@ -167,8 +185,6 @@ __device__ void wg_schedule(const WgParams& p, WgShared& s, int pair, int pairs,
     __syncthreads();
     at -= steps;
     for (int i = 0; i < warp; ++i) at += s.part[2][i];
-    if (writes && tid < 2) p.slots[2 * pair + tid] = {-1, 0};
-    __syncthreads();
     const int64_t a = max(from, at), b = min(to, at + steps);
     if (a < b) {
         const int first = (int)(a - at), last = (int)(b - at);
@@ -376,7 +392,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWgProduct) tmem_alloc(smem_addr(&s.tmem), 512);
-    wg_schedule(p, s, pair, pairs, side == 0 && p.slots);
+    wg_schedule(p, s, pair, pairs, side == 0);
     tc_fence_before();
     pair_sync();
     tc_fence_after();
@@ -661,26 +677,32 @@ static int64_t wg_tiles(int64_t n, int64_t k) {
     return (n + kWgTileN - 1) / kWgTileN * ((k + kWgTileK - 1) / kWgTileK);
 }
 
-// Pairs of blocks: one for each tile, more where few tiles have many rows (kWgMinSteps steps a pair at
-// least), at most one on each two SMs.  With groups only their average is known here.
+// How a call is split: pairs of blocks, at most one on each two SMs, and whether tiles may be cut.  One group's
+// tiles have all as many steps, and the rule of kWgCutSteps is applied here; groups' steps are known on the
+// device only.  Where tiles may be cut, a pair has at least kWgMinSteps steps on average.
 constexpr int64_t kWgMinSteps = 4;
 
-static int wg_pairs(int device, int64_t rows, int64_t n, int64_t k, int64_t groups) {
-    const int sms = std::max(2, sm_count(device));
-    const int64_t tiles = wg_tiles(n, k);
-    const int64_t steps = std::max<int64_t>(groups, (rows + kWgRows - 1) / kWgRows) * tiles;
-    const int64_t want = std::max(tiles * groups, steps / kWgMinSteps);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, sms / 2, kWgMaxPairs}));
+struct WgPlan {
+    int pairs;
+    bool cuts;
+};
+
+static WgPlan wg_plan(int device, int64_t rows, int64_t n, int64_t k, int64_t groups) {
+    const int64_t most = std::min<int64_t>(std::max(1, sm_count(device) / 2), kWgMaxPairs);
+    const int64_t tiles = wg_tiles(n, k) * groups;
+    const int64_t steps = (rows + kWgRows - 1) / kWgRows;
+    if (groups == 1) {
+        const int64_t rounds = (tiles + most - 1) / most;
+        if (rounds * steps - tiles * steps / most <= kWgCutSteps)
+            return {(int)((tiles + rounds - 1) / rounds), false};
+    }
+    const int64_t all = std::max(groups, steps) * wg_tiles(n, k);
+    return {(int)std::max<int64_t>(1, std::min(most, std::max(tiles, all / kWgMinSteps))), true};
 }
 
-// One group's tiles, all of as many steps, in whole rounds of the pairs: none is cut.
-static bool wg_cuts(int pairs, int64_t n, int64_t k, int64_t groups) {
-    return groups > 1 || wg_tiles(n, k) % pairs != 0;
-}
-
-static uint64_t wg_workspace(int pairs, int64_t n, int64_t k, int64_t groups) {
-    if (!wg_cuts(pairs, n, k, groups)) return 0;
-    return (uint64_t)pairs * 2 * (sizeof(WgSlot) + (uint64_t)kWgTileN * kWgTileK * sizeof(float));
+static uint64_t wg_workspace(const WgPlan& plan) {
+    if (!plan.cuts) return 0;
+    return (uint64_t)plan.pairs * 2 * (sizeof(WgSlot) + (uint64_t)kWgTileN * kWgTileK * sizeof(float));
 }
 
 }  // namespace aw4
@@ -689,7 +711,7 @@ using namespace aw4;
 
 extern "C" uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device) {
     if (rows <= 0 || n <= 0 || k <= 0 || groups < 1) return 0;
-    return wg_workspace(wg_pairs(device, rows, n, k, groups), n, k, groups);
+    return wg_workspace(wg_plan(device, rows, n, k, groups));
 }
 
 extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
@@ -719,10 +741,10 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     }
     if (!dy || !codes || !scales || (uintptr_t)codes % 16 || (uintptr_t)dy % 16 || ld < n || ld * 2 % 16)
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: null buffer, or rows not on 16 bytes");
-    const int pairs = wg_pairs(device, rows, n, k, groups);
-    const bool cuts = wg_cuts(pairs, n, k, groups);
-    if (cuts && (!workspace || (uintptr_t)workspace % 16 ||
-                 workspace_bytes < (int64_t)wg_workspace(pairs, n, k, groups)))
+    const WgPlan plan = wg_plan(device, rows, n, k, groups);
+    const int pairs = plan.pairs;
+    if (plan.cuts &&
+        (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)wg_workspace(plan)))
         return fail(AW4_ERR_INVALID, "aw4_weight_grad: workspace of %lld bytes is too small or misaligned",
                     (long long)workspace_bytes);
     if (!encode_tiled()) return fail(AW4_ERR_CUDA, "aw4_weight_grad: the driver has no cuTensorMapEncodeTiled");
@@ -740,7 +762,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     p.accumulate = accumulate != 0;
     p.vec_out = (uintptr_t)out % 16 == 0 && k * size % 16 == 0;
     p.partial = static_cast<float*>(workspace);
-    p.slots = cuts ? reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK) : nullptr;
+    p.slots = plan.cuts ? reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK) : nullptr;
     p.status = status;
     CUtensorMap dy_map, code_map;
     if (!encode_rows(&dy_map, dtype == AW4_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
@@ -756,7 +778,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
         note_launch();
         e = cudaGetLastError();
         if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "weight_grad launch: %s", cudaGetErrorString(e));
-        if (!cuts) return AW4_OK;
+        if (!plan.cuts) return AW4_OK;
         weight_grad_join_kernel<ot.value><<<dim3(pairs, kWgTileN / kWgSlice), 256, 0, s>>>(p, pairs);
         note_launch();
         e = cudaGetLastError();

@@ -309,6 +309,25 @@ def test_weight_grad_groups(n, k, counts):
     _check_wgrad(total, dy, x, offsets, start=start)
 
 
+@pytest.mark.parametrize("n,k,counts", [(600, 300, [4000, 10, 0, 100]),      # one long group: its tiles are cut
+                                        (130, 520, [0, 65, 2500, 1, 1900, 0]),
+                                        (5000, 4000, [2000])])               # whole rounds and cut tiles
+def test_weight_grad_cut_tiles(n, k, counts):
+    rows, offsets = sum(counts), [0]
+    for c in counts:
+        offsets.append(offsets[-1] + c)
+    x, dy = _randn(rows, k, dtype=torch.bfloat16), _randn(rows, n, seed=1, dtype=torch.bfloat16)
+    x8 = A.quantize_act8(x.to(DEV))
+    off = torch.tensor(offsets, dtype=torch.int32, device=DEV) if len(counts) > 1 else None
+    dw = A.weight_grad(dy.to(DEV), x8, off)
+    _check_wgrad(dw, dy, x, offsets if len(counts) > 1 else None)
+    again = A.weight_grad(dy.to(DEV), x8, off)
+    assert torch.equal(dw.view(torch.int16), again.view(torch.int16))
+    total = torch.ones_like(dw, dtype=torch.float32)
+    A.weight_grad(dy.to(DEV), x8, off, out=total, accumulate=True)
+    _check_wgrad(total, dy, x, offsets if len(counts) > 1 else None, start=torch.ones(total.shape))
+
+
 def test_weight_grad_bad_rows_stay_in_their_group():
     counts = [30, 50, 20, 100]
     offsets = [0, 30, 80, 100, 200]
