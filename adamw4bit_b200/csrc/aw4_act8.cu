@@ -217,8 +217,8 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
 // RMS norm: y = x r w, r = (mean(x^2) + eps)^-1/2
 // ---------------------------------------------------------------------------
 //
-// A row belongs to NT threads that hold V chunks of eight values each; NT = 32:
-// a warp a row, no barrier.  Blocks stay and walk the rows, the next row's loads on
+// A row belongs to NT threads that hold V chunks of eight values each; up to a warp
+// no barrier, and a warp has 32 / NT rows.  Blocks stay and walk the rows, the next row's loads on
 // their way while one is worked on.  The weight waits in shared memory, and the
 // backward kernel keeps its columns' sum of dy v r in registers over all its rows.
 // Two chunks a thread: a row's own cost, the sum over its threads, is then half of
@@ -233,11 +233,13 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Sum over the NT threads that share a row.  `slot` alternates so that one
 // barrier per sum is enough.
 template <int NT>
-__device__ __forceinline__ float row_sum(float v, float (*part)[NT / 32], int slot) {
-    v = warp_sum(v);
-    if constexpr (NT == 32) {
+__device__ __forceinline__ float row_sum(float v, float (*part)[NT < 64 ? 1 : NT / 32], int slot) {
+    if constexpr (NT <= 32) {
+#pragma unroll
+        for (int o = NT / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     } else {
+        v = warp_sum(v);
         if ((threadIdx.x & 31) == 0) part[slot][threadIdx.x >> 5] = v;
         __syncthreads();
         float s = 0.0f;
@@ -289,36 +291,57 @@ __device__ __forceinline__ void weight8(const float4* s, int chunks, int u, floa
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-constexpr int kNormWarps = 4;       // rows of a block at a time where a warp has a row, at most
+constexpr int kNormWarps = 4;       // warps of a block where rows belong to warps, at most
 
 // Blocks resident on an SM for that many threads of it.
 template <int NT>
 constexpr int norm_blocks(int threads) {
-    return NT == 32 ? threads / (32 * kNormWarps) : NT < threads ? threads / NT : 1;
+    return NT <= 32 ? threads / (32 * kNormWarps) : NT < threads ? threads / NT : 1;
 }
-// Forward: 1024 at 64 registers (54 us at 16384 x 4096 bf16; 58 at 768, 64 at 512).  Backward: 768 at 85 (61 us;
-// 66 at 512, 103 at 1024, where its sums spill).
-constexpr int kNormForward = 1024, kNormBackward = 768;
+
+// Which rows a thread works on: `first` and every `step` behind it, as long as `warp_first` of its warp (of its
+// block, where a row has more) is one; t: the thread's place in the row.
+template <int NT>
+struct NormWalk {
+    int64_t first, warp_first, step;
+    int t;
+    __device__ __forceinline__ NormWalk() {
+        constexpr int kRows = NT < 32 ? 32 / NT : 1;
+        const int warps = NT <= 32 ? blockDim.x >> 5 : 1, warp = NT <= 32 ? threadIdx.x >> 5 : 0;
+        step = (int64_t)gridDim.x * warps * kRows;
+        warp_first = ((int64_t)blockIdx.x * warps + warp) * kRows;
+        first = warp_first + (NT < 32 ? (threadIdx.x & 31) / NT : 0);
+        t = threadIdx.x % NT;
+    }
+};
+// Forward: 1024 threads of an SM at 64 registers (54 us at 16384 x 4096 bf16; 58 with 768, 64 with 512).
+// Backward: 768 at 85 (61 us; 66 with 512, 103 with 1024, where its sums spill); 512 where what a thread has of
+// the next row is larger, in float32 and in the two chunks of a warp's row (2047 x 1531 float32: 15 us, 17 with 768).
+constexpr int kNormForward = 1024, kNormBackwardMost = 768;
+template <int DT, int NT, int V>
+constexpr int kNormBackward = DT == AW4_F32 || (NT == 32 && V == 2) ? 512 : kNormBackwardMost;
 
 template <int DT, int NT, int V, bool WHOLE>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
+__global__ void __launch_bounds__(NT <= 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
 rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, int per_row,
                         const void* __restrict__ w, int w_dtype, float eps, const RowsOut y,
                         float* __restrict__ rstd, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                         uint8_t* __restrict__ ycodes, uint8_t* __restrict__ yscales) {
-    __shared__ float part[2][NT / 32];
+    __shared__ float part[2][NT < 64 ? 1 : NT / 32];
     extern __shared__ float4 weight_s[];
     constexpr int kChunks8 = NT * V;
-    const int held = NT == 32 ? blockDim.x >> 5 : 1;       // rows of a block at a time
-    const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * held;
-    int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
+    const NormWalk<NT> walk;
+    const int t = walk.t;
+    const int64_t step = walk.step;
+    int64_t row = walk.first;
     Raw8<DT> raw[V];
     if (row < rows)
 #pragma unroll
         for (int j = 0; j < V; ++j) raw[j] = load_raw8<DT, WHOLE>(x, row, (j * NT + t) * 8, cols);
     stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
-    for (int slot = 0; row < rows; row += step, slot ^= 1) {
+    int slot = 0;
+    for (int64_t at_row = walk.warp_first; at_row < rows; at_row += step, row += step, slot ^= 1) {
+        const bool live = NT >= 32 || row < rows;
         Raw8<DT> next[V];
         if (row + step < rows)
 #pragma unroll
@@ -334,7 +357,7 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, 
         float s0, s1;
         upk2(ss, s0, s1);
         const float r = inv_sqrt(__fmaf_rn(row_sum<NT>(s0 + s1, part, slot), inv_cols, eps));
-        if (t == 0) rstd[row] = r;
+        if (t == 0 && live) rstd[row] = r;
         uint8_t* code_row = codes + row * per_row * 8;
         uint8_t* scale_row = scales + (row * per_row >> 2);
 #pragma unroll
@@ -355,7 +378,7 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, 
                 by = a8_block<DT>(ry);
                 qy = a8_encode8(o, by);
             }
-            if (u < per_row) {
+            if (u < per_row && live) {
                 *reinterpret_cast<uint2*>(code_row + u * 8) = q;
                 if ((t & 3) == 0) scale_row[u >> 2] = (uint8_t)b.byte;
                 store_raw8<DT, WHOLE>(y, row, u * 8, cols, ry);
@@ -402,28 +425,31 @@ __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& d
 // dx = r (w dy) - v r^3 mean(v w dy); each block leaves its rows' sum of
 // dy v r in partial[blockIdx.x][cols].
 template <int DT, int NT, int V, bool WHOLE>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormBackward))
+__global__ void __launch_bounds__(NT <= 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormBackward<DT, NT, V>))
 rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols, int per_row,
                          const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                          const float* __restrict__ rstd, const void* __restrict__ w, int w_dtype,
                          const RowsOut dx, float* __restrict__ partial) {
-    __shared__ float part[2][NT / 32];
+    __shared__ float part[2][NT < 64 ? 1 : NT / 32];
     extern __shared__ float4 weight_s[];
     constexpr int kChunks8 = NT * V;
-    const int held = NT == 32 ? blockDim.x >> 5 : 1;
-    const int t = NT == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * held;
-    int64_t row = (int64_t)blockIdx.x * held + (NT == 32 ? threadIdx.x >> 5 : 0);
+    const NormWalk<NT> walk;
+    const int t = walk.t;
+    const int64_t step = walk.step;
+    int64_t row = walk.first;
     float acc[V][8];
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[j][i] = 0.0f;
-    NormRow<DT, V> now;
+    NormRow<DT, V> now = {};
     if (row < rows) load_norm_row<DT, NT, V, WHOLE>(now, dy, row, t, cols, per_row, codes, scales, rstd);
     stage_weight<NT, V>(w, w_dtype, cols, t, weight_s);
-    for (int slot = 0; row < rows; row += step, slot ^= 1) {
+    int slot = 0;
+    for (int64_t at_row = walk.warp_first; at_row < rows; at_row += step, row += step, slot ^= 1) {
+        const bool live = NT >= 32 || row < rows;
         NormRow<DT, V> next;
+        if (NT < 32) next = {};                 // a warp's last rows may not be there: zeros add nothing
         if (row + step < rows)
             load_norm_row<DT, NT, V, WHOLE>(next, dy, row + step, t, cols, per_row, codes, scales, rstd);
         const float r = now.r;
@@ -457,20 +483,26 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
             vmul8(d, d, wv);
             vmuls8(d, d, r);
             vfmas8(d, -k, v, d);
-            if (u < per_row) store_raw8<DT, WHOLE>(dx, row, u * 8, cols, narrow8<DT>(d));
+            if (u < per_row && live) store_raw8<DT, WHOLE>(dx, row, u * 8, cols, narrow8<DT>(d));
         }
         now = next;
     }
-    if constexpr (NT == 32) {
-        // the block's warps hold the same columns: added in their order
-        __shared__ float sums[V * 256];
-        for (int wi = 0; wi < held; ++wi) {
-            if ((int)(threadIdx.x >> 5) == wi)
+    if constexpr (NT <= 32) {
+        // the warp's rows and then the block's warps hold the same columns: added in their order
+        __shared__ float sums[V * NT * 8];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int o = 16; o >= NT; o >>= 1) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], o);
+        for (int wi = 0; wi < (int)(blockDim.x >> 5); ++wi) {
+            if ((int)(threadIdx.x >> 5) == wi && (threadIdx.x & 31) < NT)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        float& s = sums[(j * 32 + t) * 8 + i];
+                        float& s = sums[(j * NT + t) * 8 + i];
                         s = wi ? s + acc[j][i] : acc[j][i];
                     }
             __syncthreads();
@@ -551,6 +583,8 @@ static RowsOut rows_out(void* p, int64_t ld, int dtype) { return {static_cast<ch
 template <typename F>
 static int32_t norm_shape(int64_t cols, F f) {
     using std::integral_constant;
+    if (cols <= 64) return f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    if (cols <= 128) return f(integral_constant<int, 16>(), integral_constant<int, 1>());
     if (cols <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
     if (cols <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 2>());
     if (cols <= 1024) return f(integral_constant<int, 64>(), integral_constant<int, 2>());
@@ -575,21 +609,27 @@ static int32_t by_form(int dtype, bool whole, F f) {
 
 constexpr int64_t kNormCols = 16384;
 
-// Where a warp has a row: warps of a block, one for each SM's share of few rows.
+// Where rows belong to warps: the warps that have rows, and how many a block has of them, one for each SM's
+// share of few.
+template <int NT>
+static int64_t norm_units(int64_t rows) {
+    return NT < 32 ? (rows + 32 / NT - 1) / (32 / NT) : rows;
+}
+template <int NT>
 static int norm_warps(int device, int64_t rows) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(kNormWarps, rows / sm_count(device)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(kNormWarps, norm_units<NT>(rows) / sm_count(device)));
 }
 
 // Resident blocks, or as many as have a row: of the backward kernel also the rows of its partial sums.
 template <int NT>
 static int norm_grid(int device, int64_t rows, int threads) {
-    const int held = NT == 32 ? norm_warps(device, rows) : 1;
-    const int resident = NT == 32 ? threads / (32 * held) : norm_blocks<NT>(threads);
-    return (int)std::min<int64_t>((rows + held - 1) / held, (int64_t)sm_count(device) * resident);
+    const int held = NT <= 32 ? norm_warps<NT>(device, rows) : 1;
+    const int resident = NT <= 32 ? threads / (32 * held) : norm_blocks<NT>(threads);
+    return (int)std::min<int64_t>((norm_units<NT>(rows) + held - 1) / held, (int64_t)sm_count(device) * resident);
 }
 template <int NT>
 static int norm_threads(int device, int64_t rows) {
-    return NT == 32 ? 32 * norm_warps(device, rows) : NT;
+    return NT <= 32 ? 32 * norm_warps<NT>(device, rows) : NT;
 }
 
 template <typename K>
@@ -723,7 +763,7 @@ extern "C" uint64_t aw4_rms_norm_backward_workspace(int64_t rows, int64_t cols, 
     if (rows <= 0 || cols <= 0 || cols > kNormCols) return 0;
     int grid = 0;
     norm_shape(cols, [&](auto nt, auto) {
-        grid = norm_grid<nt.value>(device, rows, kNormBackward);
+        grid = norm_grid<nt.value>(device, rows, kNormBackwardMost);
         return (int32_t)AW4_OK;
     });
     return (uint64_t)grid * cols * sizeof(float);
@@ -763,7 +803,7 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
             auto kernel = rms_norm_backward_kernel<dt.value, nt.value, v.value, whole.value>;
             const int bytes = nt.value * v.value * 32;
             if (const int32_t rc = norm_smem(kernel, bytes)) return rc;
-            grid = norm_grid<nt.value>(device, rows, kNormBackward);
+            grid = norm_grid<nt.value>(device, rows, kNormBackward<dt.value, nt.value, v.value>);
             kernel<<<grid, norm_threads<nt.value>(device, rows), bytes, s>>>(
                 in, rows, (int)cols, 1.0f / (float)cols, (int)per_row, codes, scales, rstd, weight, weight_dtype,
                 out, workspace);

@@ -304,54 +304,45 @@ __device__ __forceinline__ void wg_convert(const char* codes, char* operand, int
     }
 }
 
-// Stores 16 bytes' worth of a row of dW: 4 float32 sums (FROM32), rounded and, with `accumulate`, added to
-// what is there, or 8 values that are rounded already.
-template <int OT, bool FROM32>
-__device__ __forceinline__ void wg_store(const WgParams& p, int64_t row_off, int k, uint4 w) {
-    constexpr int kCount = FROM32 ? 4 : 8;
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    const bool whole = p.vec_out && k + kCount <= p.k;
-    if constexpr (!FROM32) {
-        uint16_t* o = static_cast<uint16_t*>(p.out) + row_off + k;
-        if (whole) {
-            *reinterpret_cast<uint4*>(o) = w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (k + i < p.k) o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
-        }
-    } else if (OT == AW4_F32 && whole && !p.accumulate) {
-        *reinterpret_cast<uint4*>(static_cast<uint32_t*>(p.out) + row_off + k) = w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (k + i < p.k) {
-                const float f = __uint_as_float(v[i]);
-                const int64_t at = row_off + k + i;
-                Elem<OT>::store1(p.out, at, p.accumulate ? Elem<OT>::load1(p.out, at) + f : f);
-            }
-    }
-}
-
-// 32 lines of 64 bytes, a line a lane, turned in the warp's shared memory so
-// that four lanes store a line: whole sectors.  Line r is row row0 + r of group g's
-// dW, from column k on.
+// 32 lines of 64 bytes, a line a lane, turned in the warp's shared memory on
+// their way out: 16 float32 sums of a row of dW (FROM32), or 32 values rounded already.  Line r is row
+// first_row + r of dW, from column k on.  Where rows are on 16 bytes four lanes store a line in
+// vectors; else, and where sums are added to what is there, a warp stores consecutive values.
 template <int OT, bool FROM32>
 __device__ __forceinline__ void wg_store_lines(const WgParams& p, char* stage, int64_t first_row, int rows, int k,
                                                const uint32_t v[16]) {
     const int lane = threadIdx.x & 31;
+    constexpr bool kVectors = !FROM32 || OT == AW4_F32;
+    constexpr int kLine = FROM32 ? 16 : 32, kValue = FROM32 ? 4 : 2;       // values of a line, bytes of one
+    auto at = [&](int r, int byte) { return stage + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15); };
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-            make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        *reinterpret_cast<uint4*>(at(lane, c * 16)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     __syncwarp();
+    if (kVectors && p.vec_out && !p.accumulate && k + kLine <= p.k) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2), c = lane & 3;
-        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-        const int at = k + c * (FROM32 ? 4 : 8);
-        if (r < rows && at < p.k) wg_store<OT, FROM32>(p, (first_row + r) * p.k, at, w);
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
+            if (r < rows)
+                __stcs(reinterpret_cast<uint4*>(static_cast<char*>(p.out) + ((first_row + r) * p.k + k) * kValue +
+                                                (lane & 3) * 16),
+                       *reinterpret_cast<const uint4*>(at(r, (lane & 3) * 16)));
+        }
+        return;
+    }
+    const int col = lane % kLine;
+    if (k + col >= p.k) return;
+    const int end = min(rows, 32);
+#pragma unroll 4
+    for (int r = lane / kLine; r < end; r += 32 / kLine) {
+        const int64_t to = (first_row + r) * p.k + k + col;
+        if constexpr (FROM32) {
+            const float f = *reinterpret_cast<const float*>(at(r, col * 4));
+            Elem<OT>::store1(p.out, to, p.accumulate ? Elem<OT>::load1(p.out, to) + f : f);
+        } else {
+            static_cast<uint16_t*>(p.out)[to] = *reinterpret_cast<const uint16_t*>(at(r, col * 2));
+        }
     }
 }
 

@@ -141,7 +141,8 @@ def test_more_than_2_31_values():
 # ---------------------------------------------------------------------------
 
 NORM_SHAPES = [(1, 1), (1, 768), (5, 33), (64, 256), (513, 64), (37, 1000), (9, 1531), (3, 2050), (700, 2048),
-               (4, 4096), (3, 8191), (2, 16384), (2, 5, 96)]
+               (4, 4096), (3, 8191), (2, 16384), (2, 5, 96),
+               (1001, 128), (333, 24), (40000, 64)]
 
 
 def _check_norm(x, w, dy, y, saved, dx, dw, eps):
@@ -269,7 +270,8 @@ def _check_wgrad(dw, dy, x, offsets=None, start=None, rows=None):
 
 
 WGRAD = [(1, 8, 32), (16, 64, 64), (63, 8, 40), (65, 128, 256), (64, 130, 100), (200, 257, 264), (1000, 24, 33),
-         (129, 7, 1), (500, 1, 500), (300, 768, 768), (4096, 64, 96), (96, 1000, 2050)]
+         (129, 7, 1), (500, 1, 500), (300, 768, 768), (4096, 64, 96), (96, 1000, 2050),
+         (200, 600, 411), (70, 520, 412)]
 
 
 @pytest.mark.parametrize("rows,n,k", WGRAD)
