@@ -249,12 +249,12 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[NT < 64 ? 1 : NT
     }
 }
 
-// 1 / sqrt(x): the hardware's estimate and one step of Newton's method.
+// 1 / sqrt(x): the hardware's estimate and one step of Newton's method for a positive normal x.
 __device__ __forceinline__ float inv_sqrt(float x) {
+    if (!(x >= 1.17549435e-38f && x < INFINITY)) return 1.0f / sqrtf(x);
     float r;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    const float e = __fmaf_rn(-x * r, r, 1.0f);
-    return x < INFINITY ? __fmaf_rn(0.5f * r, e, r) : r;       // infinity: 0, NaN: NaN
+    return __fmaf_rn(0.5f * r, __fmaf_rn(-x * r, r, 1.0f), r);
 }
 
 // A thread's chunks of the weight as float32 in shared memory, zeros behind the

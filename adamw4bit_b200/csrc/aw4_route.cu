@@ -258,15 +258,20 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
         if (valid && row + step < rows) now_valid = valid[row + step];
         using P = Picker<DT, L, V>;
         P picker(l, lane, sorted_s, kThreads);
-        // the k largest, kept by the lanes in turn
-        int at = 0;
+        // The k largest, kept by the lanes in turn: a lane's first in registers, any further ones in shared
+        // memory.
+        int at = 0, mine_at = 0;
         const uint32_t first = picker.next(lane, at);
-        if (lane == 0) {
-            my_key[0] = first;
-            if constexpr (DT == AW4_F32) my_chosen[0] = at;
-        }
+        uint32_t mine_key = first;
+        mine_at = at;
+        const int few = min(k, L);
 #pragma unroll 2
-        for (int j = 1; j < k; ++j) {
+        for (int j = 1; j < few; ++j) {
+            const uint32_t best = picker.next(lane, at);
+            mine_key = lane == j ? best : mine_key;
+            if constexpr (DT == AW4_F32) mine_at = lane == j ? at : mine_at;
+        }
+        for (int j = few; j < k; ++j) {
             const uint32_t best = picker.next(lane, at);
             if (lane == j % L) {
                 my_key[j] = best;
@@ -286,10 +291,12 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
         if (ok)
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(l[i], inv, acc[i]);
+        const bool take = ok && lane < few && P::some(mine_key);
+        const float mine_w = take ? exp_from(P::value(mine_key), top) : 0.0f;
         float scale = inv;
         if (renormalize) {
-            float chosen_sum = 0.0f;
-            for (int j = lane; j < k; j += L)
+            float chosen_sum = mine_w;
+            for (int j = lane + L; j < k; j += L)
                 if (ok && P::some(my_key[j])) chosen_sum += exp_from(P::value(my_key[j]), top);
             chosen_sum = lanes_sum<L>(chosen_sum);
             scale = ok ? 1.0f / chosen_sum : 0.0f;
@@ -299,12 +306,18 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
                 stats[row] = make_float2(top, inv);
                 if (ok) atomicAdd(&count[experts], 1);
             }
-            for (int j = lane; j < k; j += L) {       // its own choices
-                const bool take = ok && P::some(my_key[j]);
-                const int e = take ? P::expert(my_key[j], DT == AW4_F32 ? my_chosen[j] : 0) : -1;
-                weights[picks_at + j] = take ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
-                chosen[picks_at + j] = e;
+            if (lane < few) {
+                const int e = take ? P::expert(mine_key, mine_at) : -1;
+                weights[picks_at + lane] = mine_w * scale;
+                chosen[picks_at + lane] = e;
                 if (take) atomicAdd(&count[e], 1);
+            }
+            for (int j = lane + L; j < k; j += L) {
+                const bool more = ok && P::some(my_key[j]);
+                const int e = more ? P::expert(my_key[j], DT == AW4_F32 ? my_chosen[j] : 0) : -1;
+                weights[picks_at + j] = more ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
+                chosen[picks_at + j] = e;
+                if (more) atomicAdd(&count[e], 1);
             }
         }
     }
@@ -425,30 +438,26 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         const float2 st = now_st;
         const bool ok = st.y != 0.0f;             // a NaN row is a valid one
         const int picks = dweights && in ? k : 0;
-        int at = now_at;
-        float w = now_w, d = now_d;
+        const int at = now_at;
+        const float w = now_w, d = now_d;
         float l[V];
         now.widen(l, lane, experts, ok);
         from += from_step;
         fetch(row + step, picks_at + k_step);
-        float inner = 0.0f;
-        for (int j = lane; j < picks; j += L) {
-            if (j != lane) {
-                at = chosen[picks_at + j];
-                w = weights[picks_at + j];
-                d = dweights[picks_at + j];
-            }
-            if (at >= 0) inner = __fmaf_rn(w, d, inner);
-        }
+        // up to L choices a lane has one, the one that came with the logits
+        const bool few = k <= L;
+        float inner = at >= 0 ? w * d : 0.0f;
+        if (!few)
+            for (int j = lane + L; j < picks; j += L)
+                if (chosen[picks_at + j] >= 0) inner = __fmaf_rn(weights[picks_at + j], dweights[picks_at + j], inner);
         inner = lanes_sum<L>(inner);
-        for (int j = lane; j < picks; j += L) {
-            if (k > L) {
-                at = chosen[picks_at + j];
-                w = weights[picks_at + j];
-                d = dweights[picks_at + j];
+        const float back = renormalize ? inner : 0.0f;
+        if (at >= 0) mine[at] = w * (d - back);
+        if (!few)
+            for (int j = lane + L; j < picks; j += L) {
+                const int e = chosen[picks_at + j];
+                if (e >= 0) mine[e] = weights[picks_at + j] * (dweights[picks_at + j] - back);
             }
-            if (at >= 0) mine[at] = w * (d - (renormalize ? inner : 0.0f));
-        }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -461,10 +470,12 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
 #pragma unroll
         for (int i = 0; i < V; ++i) l[i] = __fmaf_rn(l[i], share[i] - off, mine[expert_of<L>(lane, i)]);
         __syncwarp();
-        for (int j = lane; j < picks; j += L) {
-            if (k > L) at = chosen[picks_at + j];
-            if (at >= 0) mine[at] = 0.0f;
-        }
+        if (at >= 0) mine[at] = 0.0f;
+        if (!few)
+            for (int j = lane + L; j < picks; j += L) {
+                const int e = chosen[picks_at + j];
+                if (e >= 0) mine[e] = 0.0f;
+            }
         if (in)
 #pragma unroll
             for (int c = 0; c < V / 8; ++c)
