@@ -35,6 +35,8 @@ __device__ __forceinline__ int64_t warp_run(int run) {
     return ((int64_t)blockIdx.x * (kA8Threads / 32) + (threadIdx.x >> 5)) * run;
 }
 
+// A lane reads 16 bytes of bf16 and writes 8 of codes; 32 blocks' exponents leave a warp together.  Bound by
+// HBM: 8192 x 14336 bf16 in 55 us, 6.5 TB/s (72 us with a capped grid whose warps had one run or two).
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, uint8_t* __restrict__ codes,
@@ -63,6 +65,7 @@ act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, u
     store_scales(scales, unit0, units >> 2, b, lane);
 }
 
+// Bound by HBM: 8192 x 14336 bf16 in 51 us, 6.9 TB/s.
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
@@ -113,6 +116,8 @@ __device__ __forceinline__ float sigmoid(float g) {
 // 167 with two, 205 with four).
 constexpr int kGluForward = 2, kGluBackward = 1;
 
+// Reads g and u, writes h and both checkpoints (EMIT: and that of h).  Bound by HBM: 8192 x 14336 bf16 in 152 us,
+// 6.2 TB/s.
 template <int DT, bool WHOLE, bool EMIT>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols, uint32_t per_row,
@@ -164,7 +169,8 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
     }
 }
 
-// dg = dh u (s + g s (1 - s)), du = dh g s, s = sigmoid(g)
+// dg = dh u (s + g s (1 - s)), du = dh g s, s = sigmoid(g), g and u from their checkpoints.  Bound by HBM:
+// 8192 x 14336 bf16 in 149 us, 6.4 TB/s.
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row,
@@ -321,6 +327,7 @@ constexpr int kNormForward = 1024, kNormBackwardMost = 768;
 template <int DT, int NT, int V>
 constexpr int kNormBackward = DT == AW4_F32 || (NT == 32 && V == 2) ? 512 : kNormBackwardMost;
 
+// Bound by HBM: 16384 x 4096 bf16 in 54 us, 6.2 TB/s.
 template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT <= 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
 rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, int per_row,
@@ -423,7 +430,8 @@ __device__ __forceinline__ void load_norm_row(NormRow<DT, V>& n, const RowsIn& d
 }
 
 // dx = r (w dy) - v r^3 mean(v w dy); each block leaves its rows' sum of
-// dy v r in partial[blockIdx.x][cols].
+// dy v r in partial[blockIdx.x][cols].  16384 x 4096 bf16 in 61 us, 5.5 TB/s: between HBM and the
+// latency of a row's sum.
 template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT <= 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormBackward<DT, NT, V>))
 rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols, int per_row,
@@ -520,7 +528,7 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
 }
 
 // Column sums of partial[parts][cols], in a fixed order: a block has eight columns (whole sectors), 32 threads
-// share a column.
+// share a column.  444 x 4096 in 5 us, latency.
 constexpr int kSumCols = 8;
 
 template <int DT>

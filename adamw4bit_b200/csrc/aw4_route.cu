@@ -197,7 +197,9 @@ struct RowLogits {
     }
 };
 
-// Threads of a forward block: a block an SM, its sums over rows in registers.
+// One pass over the logits, a row to L lanes, so that selections and sums are shuffles.  Bound by
+// instructions (selections half of them): 65536 x 128 bf16, k = 8, in 27 us, where 10 MB a direction would take 4.
+// Threads of a block: a block an SM, its sums over rows in registers.
 template <int V>
 constexpr int kRouteThreads = V == 8 ? 1024 : V == 16 ? 512 : 256;
 
@@ -379,6 +381,8 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
     }
 }
 
+// One pass: logits, statistics and choices in, the gradient out.  65536 x 128 bf16, k = 8, in 15 us; instructions,
+// then HBM (5 us).
 constexpr int kRouteBackThreads = 256;
 template <int V>
 constexpr int kRouteBackBlocks = V == 8 ? 4 : 2;        // resident on an SM
