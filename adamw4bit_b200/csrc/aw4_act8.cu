@@ -79,6 +79,8 @@ act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restr
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
         const int64_t u = unit0 + j * 32 + lane;
+        q[j] = make_uint2(0, 0);
+        b[j] = 1;
         if (u < units) {
             q[j] = __ldcs(reinterpret_cast<const uint2*>(codes + u * 8));
             b[j] = scales[u >> 2];
@@ -87,10 +89,9 @@ act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restr
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
         const ChunkAt c = chunk_at(run, j * 32 + lane, per_row, rows);
-        if (!c.in) continue;
         float v[8];
         a8_decode8(q[j], a8_scale(b[j]), v);
-        store_raw8<DT, WHOLE>(out, c.row, c.col, cols, narrow8<DT>(v));
+        store_raw8_warp<DT, WHOLE, true>(out, c.row, c.col, cols, c.in, narrow8<DT>(v));
     }
 }
 
@@ -156,10 +157,10 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
             bh = a8_block<DT>(r);
             qh = a8_encode8(y, bh);
         }
+        store_raw8_warp<DT, WHOLE>(h, at[j].row, at[j].col, cols, at[j].in, r);
         if (!at[j].in) continue;
         *reinterpret_cast<uint2*>(gcodes + u * 8) = qg;
         *reinterpret_cast<uint2*>(ucodes + u * 8) = qu;
-        store_raw8<DT, WHOLE>(h, at[j].row, at[j].col, cols, r);
         if constexpr (EMIT) *reinterpret_cast<uint2*>(hcodes + u * 8) = qh;
         if ((lane & 3) == 0) {
             gscales[u >> 2] = (uint8_t)bg.byte;
@@ -189,6 +190,9 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
     for (int j = 0; j < kGluBackward; ++j) {
         const int64_t u = unit0 + j * 32 + lane;
         at[j] = chunk_at(run, j * 32 + lane, per_row, rows);
+        rd[j] = {};
+        qg[j] = qu[j] = make_uint2(0, 0);
+        bg[j] = bu[j] = 1;
         if (!at[j].in) continue;
         rd[j] = load_raw8<DT, WHOLE>(dh, at[j].row, at[j].col, cols);
         qg[j] = __ldcs(reinterpret_cast<const uint2*>(gcodes + u * 8));
@@ -198,7 +202,6 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
     }
 #pragma unroll
     for (int j = 0; j < kGluBackward; ++j) {
-        if (!at[j].in) continue;
         float d[8], g[8], p[8], s[8], f[8];
         widen8<DT>(rd[j], d);
         a8_decode8(qg[j], a8_scale(bg[j]), g);
@@ -214,8 +217,8 @@ swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row
         vmul8(p, p, d);
         vmul8(p, p, s);
         vmul8(g, g, d);
-        store_raw8<DT, WHOLE>(dgate, at[j].row, at[j].col, cols, narrow8<DT>(p));
-        store_raw8<DT, WHOLE>(dup, at[j].row, at[j].col, cols, narrow8<DT>(g));
+        store_raw8_warp<DT, WHOLE>(dgate, at[j].row, at[j].col, cols, at[j].in, narrow8<DT>(p));
+        store_raw8_warp<DT, WHOLE>(dup, at[j].row, at[j].col, cols, at[j].in, narrow8<DT>(g));
     }
 }
 
@@ -385,10 +388,10 @@ rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, 
                 by = a8_block<DT>(ry);
                 qy = a8_encode8(o, by);
             }
+            store_raw8_warp<DT, WHOLE>(y, row, u * 8, cols, u < per_row && live, ry);
             if (u < per_row && live) {
                 *reinterpret_cast<uint2*>(code_row + u * 8) = q;
                 if ((t & 3) == 0) scale_row[u >> 2] = (uint8_t)b.byte;
-                store_raw8<DT, WHOLE>(y, row, u * 8, cols, ry);
                 if (ycodes) {
                     *reinterpret_cast<uint2*>(ycodes + row * per_row * 8 + u * 8) = qy;
                     if ((t & 3) == 0) yscales[(row * per_row + u) >> 2] = (uint8_t)by.byte;
@@ -491,7 +494,7 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
             vmul8(d, d, wv);
             vmuls8(d, d, r);
             vfmas8(d, -k, v, d);
-            if (u < per_row && live) store_raw8<DT, WHOLE>(dx, row, u * 8, cols, narrow8<DT>(d));
+            store_raw8_warp<DT, WHOLE>(dx, row, u * 8, cols, u < per_row && live, narrow8<DT>(d));
         }
         now = next;
     }
@@ -554,11 +557,6 @@ column_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* 
 static bool known_dtype(int dtype) { return dtype >= AW4_F32 && dtype <= AW4_F16; }
 static int size_of(int dtype) { return dtype == AW4_F32 ? 4 : 2; }
 
-// Whether whole chunks of eight values of every row start on 16 bytes.
-static bool vec_ok(const void* p, int64_t ld, int dtype) {
-    return (uintptr_t)p % 16 == 0 && (ld * size_of(dtype)) % 16 == 0;
-}
-
 static int32_t check_matrix(const char* what, int dtype, int64_t rows, int64_t cols) {
     if (!known_dtype(dtype)) return fail(AW4_ERR_INVALID, "%s: bad dtype %d", what, dtype);
     if (rows < 0 || cols < 0) return fail(AW4_ERR_INVALID, "%s: negative size", what);
@@ -583,9 +581,9 @@ static unsigned run_grid(int64_t units, int run) {
 
 static RowsIn rows_in(const void* p, int64_t rows, int64_t cols, int64_t ld, int dtype) {
     const char* base = static_cast<const char*>(p);
-    return {base, base + ((rows - 1) * ld + cols) * size_of(dtype), ld, vec_ok(p, ld, dtype)};
+    return {base, base + ((rows - 1) * ld + cols) * size_of(dtype), ld, rows_on(p, ld, dtype, 16)};
 }
-static RowsOut rows_out(void* p, int64_t ld, int dtype) { return {static_cast<char*>(p), ld, vec_ok(p, ld, dtype)}; }
+static RowsOut rows_out(void* p, int64_t ld, int dtype) { return {static_cast<char*>(p), ld, rows_on(p, ld, dtype, 16)}; }
 
 // A row's threads and chunks of eight.
 template <typename F>
@@ -661,7 +659,7 @@ extern "C" int32_t aw4_act8_quantize(const void* x, int32_t dtype, int64_t rows,
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
     const RowsIn in = rows_in(x, rows, cols, ld, dtype);
-    return by_form(dtype, in.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    return by_form(dtype, rows_whole(x, ld, cols, dtype), [&](auto dt, auto whole) {
         act8_quantize_kernel<dt.value, whole.value>
             <<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(in, rows, (int)cols, per_row,
                                                                                      codes, scales);
@@ -680,7 +678,7 @@ extern "C" int32_t aw4_act8_dequantize(const uint8_t* codes, const uint8_t* scal
     if (!guard.ok()) return fail(AW4_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const uint32_t per_row = chunks_per_row(cols);
     const RowsOut to = rows_out(out, ld, dtype);
-    return by_form(dtype, to.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    return by_form(dtype, rows_whole(out, ld, cols, dtype), [&](auto dt, auto whole) {
         act8_dequantize_kernel<dt.value, whole.value>
             <<<run_grid(rows * per_row, kRun), kA8Threads, 0, (cudaStream_t)stream>>>(codes, scales, rows, (int)cols,
                                                                                      per_row, to);
@@ -703,7 +701,9 @@ extern "C" int32_t aw4_swiglu_forward(const void* gate, const void* up, int32_t 
     const RowsIn g = rows_in(gate, rows, cols, ld_gate, dtype), u = rows_in(up, rows, cols, ld_up, dtype);
     const RowsOut o = rows_out(h, cols, dtype);
     const unsigned grid = run_grid(rows * per_row, 32 * kGluForward);
-    return by_form(dtype, g.vec && u.vec && o.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    const bool all_whole = rows_whole(gate, ld_gate, cols, dtype) && rows_whole(up, ld_up, cols, dtype) &&
+                           rows_whole(h, cols, cols, dtype);
+    return by_form(dtype, all_whole, [&](auto dt, auto whole) {
         if (hcodes)
             swiglu_forward_kernel<dt.value, whole.value, true><<<grid, kA8Threads, 0, (cudaStream_t)stream>>>(
                 g, u, rows, (int)cols, per_row, o, gcodes, gscales, ucodes, uscales, hcodes, hscales);
@@ -728,7 +728,9 @@ extern "C" int32_t aw4_swiglu_backward(const void* dh, int32_t dtype, int64_t ro
     const uint32_t per_row = chunks_per_row(cols);
     const RowsIn in = rows_in(dh, rows, cols, ld_dh, dtype);
     const RowsOut dg = rows_out(dgate, ld_out, dtype), du = rows_out(dup, ld_out, dtype);
-    return by_form(dtype, in.vec && dg.vec && du.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    const bool all_whole = rows_whole(dh, ld_dh, cols, dtype) && rows_whole(dgate, ld_out, cols, dtype) &&
+                           rows_whole(dup, ld_out, cols, dtype);
+    return by_form(dtype, all_whole, [&](auto dt, auto whole) {
         swiglu_backward_kernel<dt.value, whole.value>
             <<<run_grid(rows * per_row, 32 * kGluBackward), kA8Threads, 0, (cudaStream_t)stream>>>(
                 in, rows, (int)cols, per_row, gcodes, gscales, ucodes, uscales, dg, du);
@@ -754,7 +756,8 @@ extern "C" int32_t aw4_rms_norm_forward(const void* x, int32_t dtype, int64_t ro
     const uint32_t per_row = chunks_per_row(cols);
     const RowsIn in = rows_in(x, rows, cols, ld, dtype);
     const RowsOut out = rows_out(y, cols, dtype);
-    return by_form(dtype, in.vec && out.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    const bool all_whole = rows_whole(x, ld, cols, dtype) && rows_whole(y, cols, cols, dtype);
+    return by_form(dtype, all_whole, [&](auto dt, auto whole) {
         return norm_shape(cols, [&](auto nt, auto v) {
             auto kernel = rms_norm_forward_kernel<dt.value, nt.value, v.value, whole.value>;
             const int bytes = nt.value * v.value * 32;
@@ -806,7 +809,8 @@ extern "C" int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t 
     int grid = 0;
     const RowsIn in = rows_in(dy, rows, cols, ld, dtype);
     const RowsOut out = rows_out(dx, cols, dtype);
-    const int32_t rc = by_form(dtype, in.vec && out.vec && cols % 8 == 0, [&](auto dt, auto whole) {
+    const bool all_whole = rows_whole(dy, ld, cols, dtype) && rows_whole(dx, cols, cols, dtype);
+    const int32_t rc = by_form(dtype, all_whole, [&](auto dt, auto whole) {
         return norm_shape(cols, [&](auto nt, auto v) {
             auto kernel = rms_norm_backward_kernel<dt.value, nt.value, v.value, whole.value>;
             const int bytes = nt.value * v.value * 32;

@@ -36,9 +36,9 @@ struct Raw8 {
 };
 
 // Rows of a matrix in memory.  `vec`: every row starts on 16 bytes.  Kernels come in two
-// forms: WHOLE where that holds for all their matrices and rows are whole chunks of eight, so that
-// every access is one of vectors and the code for the others is not in the way (router backward:
-// 400 instructions a row without).
+// forms: WHOLE where all their matrices' rows are whole chunks of eight that start on a chunk's size (16 bytes, 32 in
+// float32), so that an access is one vector and the code for the others is not in the way (router
+// backward: 400 instructions a row without).
 struct RowsIn {
     const char* base;
     const char* end;      // behind the last value
@@ -51,15 +51,30 @@ struct RowsOut {
     bool vec;
 };
 
+inline bool rows_on(const void* p, int64_t ld, int dtype, int bytes) {
+    return (uintptr_t)p % bytes == 0 && ld * (dtype == AW4_F32 ? 4 : 2) % bytes == 0;
+}
+// Whether a matrix can take the WHOLE form.
+inline bool rows_whole(const void* p, int64_t ld, int64_t cols, int dtype) {
+    return cols % 8 == 0 && rows_on(p, ld, dtype, dtype == AW4_F32 ? 32 : 16);
+}
+
 // Values [col, col + 8) of the row that has its column `col` at p; zeros from `cols` on.
 template <int DT, bool WHOLE>
 __device__ __forceinline__ Raw8<DT> load_raw8_at(const RowsIn& m, const char* p, int col, int cols) {
     constexpr int kSize = Elem<DT>::kBytes, kWords = kSize * 2;
     Raw8<DT> r;
-    if constexpr (WHOLE) {
+    if constexpr (WHOLE && DT == AW4_F32) {
+        uint32_t* v = reinterpret_cast<uint32_t*>(r.w);
 #pragma unroll
-        for (int i = 0; i < kSize / 2; ++i)
-            r.w[i] = col < cols ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 8; ++i) v[i] = 0;
+        if (col < cols)
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                         : "l"(p));
+        return r;
+    } else if constexpr (WHOLE) {
+        r.w[0] = col < cols ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
         return r;
     }
     uint32_t* w = reinterpret_cast<uint32_t*>(r.w);
@@ -112,13 +127,17 @@ __device__ __forceinline__ Raw8<DT> load_raw8(const RowsIn& m, int64_t row, int 
 template <int DT, bool WHOLE>
 __device__ __forceinline__ void store_raw8_at(const RowsOut& m, char* p, int col, int cols, const Raw8<DT>& r) {
     constexpr int kSize = Elem<DT>::kBytes;
-    if constexpr (WHOLE) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+    if constexpr (WHOLE && DT == AW4_F32) {
         if (col < cols)
-#pragma unroll
-            for (int i = 0; i < kSize / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                         ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        return;
+    } else if constexpr (WHOLE) {
+        if (col < cols) __stcs(reinterpret_cast<uint4*>(p), r.w[0]);
         return;
     }
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
     if (col + 8 <= cols) {
         if (m.vec) {
 #pragma unroll
@@ -212,6 +231,58 @@ __device__ __forceinline__ Raw8<DT> narrow8(const float v[8]) {
 template <int DT, bool WHOLE>
 __device__ __forceinline__ void store_raw8(const RowsOut& m, int64_t row, int col, int cols, const Raw8<DT>& r) {
     store_raw8_at<DT, WHOLE>(m, m.base + (row * m.ld + col) * Elem<DT>::kBytes, col, cols, r);
+}
+
+// The same by a whole warp, lanes with `in` storing.  Where its lanes hold consecutive whole chunks of a row
+// that starts off 16 bytes, each takes what it lacks to whole aligned vectors from the next lane (TURN).  In
+// float32 that pays everywhere (8192 x 8191 read back and forth 220 -> 135 us), in 16 bits where a
+// kernel does little else (118 -> 104 us; gated activation 276 -> 305).
+template <int DT, bool WHOLE, bool TURN = DT == AW4_F32>
+__device__ __forceinline__ void store_raw8_warp(const RowsOut& m, int64_t row, int col, int cols, bool in,
+                                                const Raw8<DT>& r) {
+    constexpr int kSize = Elem<DT>::kBytes, kWords = 2 * kSize;
+    if constexpr (WHOLE) {
+        if (in) store_raw8<DT, true>(m, row, col, cols, r);
+    } else if constexpr (!TURN) {
+        if (in) store_raw8<DT, false>(m, row, col, cols, r);
+    } else {
+        const int lane = threadIdx.x & 31;
+        char* p = m.base + (row * m.ld + col) * kSize;
+        const char* first = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, (unsigned long long)p, 0));
+        if (m.vec || !__all_sync(0xffffffffu, in && col + 8 <= cols && p == first + lane * 8 * kSize)) {
+            if (in) store_raw8_at<DT, false>(m, p, col, cols, r);
+            return;
+        }
+        const int head = (int)((16 - ((uintptr_t)p & 15)) & 15);       // bytes before the first aligned vector
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+        uint32_t v[kWords + 4];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) v[i] = w[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[kWords + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+        if (head & 8)
+#pragma unroll
+            for (int i = 0; i + 2 < kWords + 4; ++i) v[i] = v[i + 2];
+        if (head & 4)
+#pragma unroll
+            for (int i = 0; i + 1 < kWords + 4; ++i) v[i] = v[i + 1];
+        if (kSize == 2 && (head & 2))
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 16);
+        if (lane < 31 || head == 0)
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i)
+                __stcs(reinterpret_cast<uint4*>(p + head) + i,
+                       make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        // the first lane's values before its first vector, the last lane's behind it
+        if (head && (lane == 0 || lane == 31))
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane == 0 ? i * kSize < head : i * kSize >= head) {
+                    if constexpr (DT == AW4_F32) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+                    else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+                }
+    }
 }
 
 // Larger magnitude of two words' values (its sign is not meaningful); a NaN is above every number.

@@ -543,13 +543,9 @@ static int route_grid(int device, int64_t rows, int experts) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, sm_count(device)));
 }
 
-static bool route_vec(const void* p, int64_t ld, int dtype) {
-    return (uintptr_t)p % 16 == 0 && ld * (dtype == AW4_F32 ? 4 : 2) % 16 == 0;
-}
-
 static RowsIn route_rows(const void* p, int64_t rows, int experts, int64_t ld, int dtype) {
     const char* base = static_cast<const char*>(p);
-    return {base, base + ((rows - 1) * ld + experts) * (dtype == AW4_F32 ? 4 : 2), ld, route_vec(p, ld, dtype)};
+    return {base, base + ((rows - 1) * ld + experts) * (dtype == AW4_F32 ? 4 : 2), ld, rows_on(p, ld, dtype, 16)};
 }
 
 }  // namespace aw4
@@ -595,7 +591,7 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
                                              Picker<dt.value, lanes.value, v.value>::kShared * kThreads,
                                          kThreads / 32 * v.value * lanes.value);
             const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
-            return route_form<v.value>(in.vec && experts == lanes.value * v.value, [&](auto whole) {
+            return route_form<v.value>(rows_whole(logits, ld, experts, dtype) && experts == lanes.value * v.value, [&](auto whole) {
             auto kernel = route_forward_kernel<dt.value, lanes.value, v.value, whole.value>;
             const int bytes = (experts + 1 + choices) * 4;
             if (bytes > 40 * 1024) {
@@ -631,8 +627,9 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
             const int grid = (int)std::min<int64_t>((rows + per - 1) / per,
                                                    (int64_t)sm_count(device) * kRouteBackBlocks<v.value>);
             const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
-            const RowsOut out = {static_cast<char*>(dlogits), experts, route_vec(dlogits, experts, dtype)};
-            return route_form<v.value>(in.vec && out.vec && experts == lanes.value * v.value, [&](auto whole) {
+            const RowsOut out = {static_cast<char*>(dlogits), experts, rows_on(dlogits, experts, dtype, 16)};
+            return route_form<v.value>(rows_whole(logits, ld, experts, dtype) && rows_whole(dlogits, experts, experts, dtype) &&
+                                           experts == lanes.value * v.value, [&](auto whole) {
             route_backward_kernel<dt.value, lanes.value, v.value, whole.value>
                 <<<grid, kRouteBackThreads, 0, (cudaStream_t)stream>>>(
                     in, rows, experts, k, renormalize != 0, weights, chosen, reinterpret_cast<const float2*>(stats),
