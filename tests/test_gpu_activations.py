@@ -142,7 +142,7 @@ def test_more_than_2_31_values():
 
 NORM_SHAPES = [(1, 1), (1, 768), (5, 33), (64, 256), (513, 64), (37, 1000), (9, 1531), (3, 2050), (700, 2048),
                (4, 4096), (3, 8191), (2, 16384), (2, 5, 96),
-               (1001, 128), (333, 24), (40000, 64)]
+               (1001, 128), (333, 24), (40000, 64), (130, 1280), (70, 2560), (40, 5120), (30, 6144), (20, 7168), (10, 12288)]
 
 
 def _check_norm(x, w, dy, y, saved, dx, dw, eps):
