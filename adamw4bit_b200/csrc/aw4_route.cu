@@ -199,9 +199,11 @@ struct RowLogits {
 
 // One pass over the logits, a row to L lanes, so that selections and sums are shuffles.  Bound by
 // instructions (selections half of them): 65536 x 128 bf16, k = 8, in 27 us, where 10 MB a direction would take 4.
-// Threads of a block: a block an SM, its sums over rows in registers.
+// Blocks of T threads stay, one an SM, their sums over rows in registers: 1024 threads, or what registers
+// allow from 257 experts on; 256 where 1024 would leave SMs without a row (48 x 8: 4.5 us for 6.5).
+constexpr int kRouteFew = 256;
 template <int V>
-constexpr int kRouteThreads = V == 8 ? 1024 : V == 16 ? 512 : 256;
+constexpr int kRouteMost = V == 8 ? 1024 : V == 16 ? 512 : 256;
 
 // What the blocks of a call add up, zero before it.  The sums of p are whole
 // numbers of 2^-32, so that the order of the additions does not matter; a
@@ -217,13 +219,13 @@ __host__ __device__ constexpr int64_t route_totals_bytes(int experts) {
     return (int64_t)sizeof(RouteTotals) + 12 * (int64_t)experts;
 }
 
-template <int DT, int L, int V, bool WHOLE>
-__global__ void __launch_bounds__(kRouteThreads<V>, 1)
+template <int DT, int L, int V, bool WHOLE, int T>
+__global__ void __launch_bounds__(T, V == 8 ? 1024 / T : 1)
 route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, const uint8_t* __restrict__ valid,
                      bool renormalize, float* __restrict__ weights, int32_t* __restrict__ chosen,
                      float2* __restrict__ stats, RouteTotals* __restrict__ totals, int32_t* __restrict__ counts,
                      int32_t* __restrict__ valid_rows, float* __restrict__ balance) {
-    constexpr int kThreads = kRouteThreads<V>, kRows = kThreads / L;
+    constexpr int kThreads = T, kRows = kThreads / L;
     extern __shared__ int32_t smem[];
     __shared__ float scratch[kThreads / 32];
     __shared__ int is_last;
@@ -536,11 +538,15 @@ static int route_lanes(int experts) {
     return lanes;
 }
 
-// Blocks of the forward kernel and threads of each: one an SM, or as many as have a row.
-static int route_threads(int experts) { return experts <= 256 ? 1024 : experts <= 512 ? 512 : 256; }
+// Threads of the forward kernel's blocks, and blocks: as many as have a row, at most one an SM (of 256 threads four).
+static int route_threads(int device, int64_t rows, int experts) {
+    const int most = experts <= 256 ? kRouteMost<8> : experts <= 512 ? kRouteMost<16> : kRouteMost<32>;
+    return rows * route_lanes(experts) / most < sm_count(device) ? kRouteFew : most;
+}
 static int route_grid(int device, int64_t rows, int experts) {
-    const int per = route_threads(experts) / route_lanes(experts);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, sm_count(device)));
+    const int threads = route_threads(device, rows, experts), per = threads / route_lanes(experts);
+    const int64_t resident = (int64_t)sm_count(device) * (threads == kRouteFew && experts <= 256 ? 4 : 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, resident));
 }
 
 static RowsIn route_rows(const void* p, int64_t rows, int experts, int64_t ld, int dtype) {
@@ -585,26 +591,34 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
     }
     return route_by_dtype(dtype, [&](auto dt) {
         return route_shape(experts, [&](auto lanes, auto v) {
-            constexpr int kThreads = kRouteThreads<v.value>;
-            // choices of the rows in work, later the warps' sums
-            const int choices = std::max(2 * (kThreads / lanes.value) * k +
-                                             Picker<dt.value, lanes.value, v.value>::kShared * kThreads,
-                                         kThreads / 32 * v.value * lanes.value);
             const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
-            return route_form<v.value>(rows_whole(logits, ld, experts, dtype) && experts == lanes.value * v.value, [&](auto whole) {
-            auto kernel = route_forward_kernel<dt.value, lanes.value, v.value, whole.value>;
-            const int bytes = (experts + 1 + choices) * 4;
-            if (bytes > 40 * 1024) {
-                const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-                if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
-            }
-            kernel<<<grid, kThreads, bytes, s>>>(in, rows, experts, k, valid,
-                                                 renormalize != 0, weights, chosen, reinterpret_cast<float2*>(stats),
-                                                 static_cast<RouteTotals*>(workspace), counts, valid_rows, balance);
-            note_launch();
-            const cudaError_t e = cudaGetLastError();
-            return e == cudaSuccess ? (int32_t)AW4_OK
-                                    : fail(AW4_ERR_CUDA, "route_forward launch: %s", cudaGetErrorString(e));
+            const bool all_whole = rows_whole(logits, ld, experts, dtype) && experts == lanes.value * v.value;
+            return route_form<v.value>(all_whole, [&](auto whole) {
+                auto go = [&](auto threads) -> int32_t {
+                    constexpr int kThreads = threads.value;
+                    // choices of the rows in work, later the warps' sums
+                    const int choices = std::max(2 * (kThreads / lanes.value) * k +
+                                                     Picker<dt.value, lanes.value, v.value>::kShared * kThreads,
+                                                 kThreads / 32 * v.value * lanes.value);
+                    auto kernel = route_forward_kernel<dt.value, lanes.value, v.value, whole.value, kThreads>;
+                    const int bytes = (experts + 1 + choices) * 4;
+                    if (bytes > 40 * 1024) {
+                        const cudaError_t e =
+                            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+                        if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
+                    }
+                    kernel<<<grid, kThreads, bytes, s>>>(in, rows, experts, k, valid, renormalize != 0, weights, chosen,
+                                                         reinterpret_cast<float2*>(stats),
+                                                         static_cast<RouteTotals*>(workspace), counts, valid_rows,
+                                                         balance);
+                    note_launch();
+                    const cudaError_t e = cudaGetLastError();
+                    return e == cudaSuccess ? (int32_t)AW4_OK
+                                            : fail(AW4_ERR_CUDA, "route_forward launch: %s", cudaGetErrorString(e));
+                };
+                if (route_threads(device, rows, experts) == kRouteFew)
+                    return go(std::integral_constant<int, kRouteFew>());
+                return go(std::integral_constant<int, kRouteMost<v.value>>());
             });
         });
     });
