@@ -45,8 +45,8 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 template <int L>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    // a whole warp's in one instruction (65536 x 256 bf16, k = 8: 47 -> 41 us); half warps' by it
-    // take longer than by shuffles (128 experts: 28.7 -> 30.8)
+    // a whole warp's in one instruction (16384 x 1024, k = 8: 74 us by shuffles, 67); that of half a
+    // warp takes longer so (65536 x 128 by 16 lanes: 28.7 us, 30.8)
     if constexpr (L == 32) {
         v = __reduce_max_sync(0xffffffffu, v);
     } else {
@@ -64,127 +64,114 @@ __device__ __forceinline__ float exp_from(float l, float top) {
     return r;
 }
 
-// The logits' order as unsigned integers: -0 = +0, NaN on top, 0 for a logit that takes no part.
-constexpr uint32_t kKeyNegInf = 0x007fffffu;
-
-__device__ __forceinline__ uint32_t order_key(float l) {
-    const uint32_t u = __float_as_uint(l + 0.0f);                     // -0 + 0 = +0
-    const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    return l != l ? 0xffffffffu : k;
+// Sorts eight words, the largest first (Batcher's odd-even merge).
+template <typename K>
+__device__ __forceinline__ void sort8(K key[8]) {
+    constexpr int kA[19] = {0, 2, 4, 6, 0, 1, 4, 5, 1, 5, 0, 1, 2, 3, 2, 3, 1, 3, 5};
+    constexpr int kB[19] = {1, 3, 5, 7, 2, 3, 6, 7, 2, 6, 4, 5, 6, 7, 4, 5, 2, 4, 6};
+#pragma unroll
+    for (int i = 0; i < 19; ++i) {
+        const K a = key[kA[i]], b = key[kB[i]];
+        key[kA[i]] = a > b ? a : b;
+        key[kB[i]] = a > b ? b : a;
+    }
 }
-// Takes a row's logits from the largest down.  float32: the largest key left by a scan and
-// shuffles, then the lowest lane and place that has it by a ballot.
-template <int DT, int L, int V, bool kPacked = DT != AW4_F32>
-struct Picker {
-    uint32_t key[V];
-    static constexpr int kShared = 0;      // words of shared memory a thread
-    __device__ __forceinline__ Picker(const float l[V], int, uint32_t*, int) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = order_key(l[i]);
-    }
-    // The next key and the expert that has it; a key of 0 has none.
-    __device__ __forceinline__ uint32_t next(int lane, int& at) {
-        uint32_t best = key[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) best = max(best, key[i]);
-        best = lanes_max<L>(best);
-        at = 0x7fffffff;
-#pragma unroll
-        for (int i = V - 1; i >= 0; --i)
-            if (key[i] == best) at = expert_of<L>(lane, i);
-        if constexpr (V == 8) {
-            // lanes hold ascending experts: the first lane that has it
-            const uint32_t here = (threadIdx.x & 31) & ~(L - 1);
-            uint32_t has = __ballot_sync(0xffffffffu, at != 0x7fffffff) >> here;
-            if constexpr (L < 32) has &= (1u << L) - 1;
-            at = __shfl_sync(0xffffffffu, at, here + __ffs(has) - 1);
-        } else {
-#pragma unroll
-            for (int o = L / 2; o; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (at == expert_of<L>(lane, i)) key[i] = 0;
-        return best;
-    }
-    static __device__ __forceinline__ bool some(uint32_t best) { return best > kKeyNegInf; }
-    static __device__ __forceinline__ int expert(uint32_t, int at) { return at; }
-    static __device__ __forceinline__ float value(uint32_t k) {
-        if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
-        return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-    }
-};
 
-// 16-bit logits: their order in the upper half of a word and the index, counted
-// down, in the lower.  Words are then all different and one maximum gives both.
-// Eight of a lane are sorted once (Batcher's odd-even merge) and wait in shared memory; a
-// lane holds its largest, and the lane that had the row's takes its next.
+// Takes a row's logits from the largest down.  A key holds a logit's order as an unsigned integer (-0 = +0, NaN on
+// top) above its index counted down, so keys are all different and the largest is also the lowest
+// index's: one word for 16-bit logits, two for float32.  None is 0.
+// Each eight of a lane are sorted once and wait in shared memory; a lane holds its lists' largest, and the
+// list that had the row's takes its next.
 template <int DT, int L, int V>
-struct Picker<DT, L, V, true> {
-    static constexpr int kShared = V == 8 ? 8 : 0;
-    uint32_t key[V];
-    uint32_t* rest;      // the next of this lane's keys
+struct Picker {
+    using Key = std::conditional_t<DT == AW4_F32, unsigned long long, uint32_t>;
+    static constexpr int kLists = V / 8, kShared = V * (int)sizeof(Key) / 4;      // words of shared memory a thread
+    Key head[kLists];
+    Key* rest[kLists];      // the next of the list's keys, 0 behind them
     int stride;
 
-    __device__ __forceinline__ Picker(const float l[V], int lane, uint32_t* shared, int threads) {
-        rest = shared + threadIdx.x;
+    __device__ __forceinline__ Picker(const Raw8<DT> raw[kLists], int lane, uint32_t* shared, int threads) {
         stride = threads;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = expert_of<L>(lane, i);
-            const float z = l[i] + 0.0f;
-            const uint32_t u = DT == AW4_BF16 ? __float_as_uint(z)
-                                              : (uint32_t)__half_as_ushort(__float2half_rn(z)) << 16;
-            uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-            k = l[i] != l[i] ? 0xffffffffu : k;
-            key[i] = (k & 0xffff0000u) | (0xffffu - e);
-        }
-        if constexpr (V == 8) {
-            constexpr int kA[19] = {0, 2, 4, 6, 0, 1, 4, 5, 1, 5, 0, 1, 2, 3, 2, 3, 1, 3, 5};
-            constexpr int kB[19] = {1, 3, 5, 7, 2, 3, 6, 7, 2, 6, 4, 5, 6, 7, 4, 5, 2, 4, 6};
+        for (int c = 0; c < kLists; ++c) {
+            Key key[8];
+            keys(raw[c], 0xffffu - expert_of<L>(lane, c * 8), key);
+            sort8(key);
+            rest[c] = reinterpret_cast<Key*>(shared) + c * 8 * threads + threadIdx.x;
+            head[c] = key[0];
 #pragma unroll
-            for (int c = 0; c < 19; ++c) {
-                const uint32_t a = key[kA[c]], b = key[kB[c]];
-                key[kA[c]] = max(a, b);
-                key[kB[c]] = min(a, b);
-            }
-#pragma unroll
-            for (int i = 1; i < V; ++i) rest[(i - 1) * stride] = key[i];
-            rest[(V - 1) * stride] = 0;
+            for (int i = 1; i < 8; ++i) rest[c][(i - 1) * stride] = key[i];
+            rest[c][7 * stride] = 0;
         }
     }
-    __device__ __forceinline__ uint32_t next(int, int&) {
-        uint32_t mine = key[0];
-        if constexpr (V != 8)
+    // low: what the first one's index counts down to
+    static __device__ __forceinline__ void keys(const Raw8<DT>& raw, uint32_t low, Key key[8]) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(raw.w);
+        if constexpr (DT == AW4_F32) {
 #pragma unroll
-            for (int i = 1; i < V; ++i) mine = max(mine, key[i]);
-        const uint32_t best = lanes_max<L>(mine);
-        if constexpr (V == 8) {
-            if (mine == best && best) {
-                key[0] = *rest;
-                rest += stride;
+            for (int i = 0; i < 8; ++i) {
+                const float z = __uint_as_float(w[i]) + 0.0f;                     // -0 + 0 = +0
+                const uint32_t u = __float_as_uint(z);
+                const uint32_t k = z != z ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+                key[i] = (unsigned long long)k << 32 | (low - i);
             }
         } else {
+            // two logits at once; their sums with 0 turn -0 to +0 and a NaN to 0x7fff, the largest of all
+            uint32_t two = low | (low - 1) << 16;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (key[i] == best) key[i] = 0;
+            for (int i = 0; i < 4; ++i) {
+                uint32_t u;
+                if constexpr (DT == AW4_BF16) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(w[i]), "r"(0));
+                else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(u) : "r"(w[i]), "r"(0));
+                uint32_t negative;      // all ones in the half of a number with a sign
+                asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(negative) : "r"(u));
+                const uint32_t k = u ^ (negative | 0x80008000u);
+                key[2 * i] = __byte_perm(two, k, 0x5410);
+                key[2 * i + 1] = __byte_perm(two, k, 0x7632);
+                two -= 0x00020002u;
+            }
         }
+    }
+    __device__ __forceinline__ Key next() {
+        Key mine = head[0];
+#pragma unroll
+        for (int c = 1; c < kLists; ++c) mine = mine > head[c] ? mine : head[c];
+        Key best;
+        if constexpr (DT == AW4_F32) {
+            const uint32_t top = lanes_max<L>((uint32_t)(mine >> 32));
+            best = (unsigned long long)top << 32 | lanes_max<L>((uint32_t)(mine >> 32) == top ? (uint32_t)mine : 0u);
+        } else {
+            best = lanes_max<L>(mine);
+        }
+#pragma unroll
+        for (int c = 0; c < kLists; ++c)
+            if (head[c] == best) {
+                head[c] = *rest[c];
+                rest[c] += stride;
+            }
         return best;
     }
-    static __device__ __forceinline__ bool some(uint32_t best) {
-        return (best >> 16) > (DT == AW4_BF16 ? 0x007fu : 0x03ffu);         // above -inf
+    // whether it is above -inf
+    static __device__ __forceinline__ bool some(Key best) {
+        if constexpr (DT == AW4_F32) return (uint32_t)(best >> 32) > 0x007fffffu;
+        else return (best >> 16) > (DT == AW4_BF16 ? 0x007fu : 0x03ffu);
     }
-    static __device__ __forceinline__ int expert(uint32_t best, int) { return (int)(0xffffu - (best & 0xffffu)); }
-    static __device__ __forceinline__ float value(uint32_t best) {
-        const uint32_t top = best >> 16;
-        if (top == 0xffffu) return __uint_as_float(0x7fc00000u);
-        const uint32_t u = (top & 0x8000u) ? top & 0x7fffu : ~top & 0xffffu;
-        return DT == AW4_BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+    static __device__ __forceinline__ int expert(Key best) { return (int)(0xffffu - ((uint32_t)best & 0xffffu)); }
+    static __device__ __forceinline__ float value(Key best) {
+        if constexpr (DT == AW4_F32) {
+            const uint32_t k = (uint32_t)(best >> 32);
+            if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+            return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+        } else {
+            const uint32_t top = best >> 16;
+            if (top == 0xffffu) return __uint_as_float(0x7fc00000u);
+            const uint32_t u = (top & 0x8000u) ? top & 0x7fffu : ~top & 0xffffu;
+            return DT == AW4_BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+        }
     }
 };
 
-// A row's logits as loaded, and widened with -inf in the place of those that take no part.  WHOLE: rows of
-// V L experts on 16 bytes.
+// A row's logits as loaded.  WHOLE: rows of V L experts on 16 bytes.
 template <int DT, int L, int V, bool WHOLE>
 struct RowLogits {
     Raw8<DT> raw[V / 8];
@@ -194,22 +181,40 @@ struct RowLogits {
         for (int c = 0; c < V / 8; ++c)
             raw[c] = load_raw8_at<DT, WHOLE>(logits, p + c * L * 8 * Elem<DT>::kBytes, (c * L + lane) * 8, in ? experts : 0);
     }
-    __device__ __forceinline__ void widen(float l[V], int lane, int experts, bool in) const {
+    // -inf in the place of those that take no part
+    __device__ __forceinline__ void mask(int lane, int experts, bool in) {
+        constexpr uint32_t kNegInf = DT == AW4_F32 ? 0xff800000u : DT == AW4_BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+        for (int c = 0; c < V / 8; ++c) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(raw[c].w);
+            const int have = !in ? 0 : WHOLE ? 8 : experts - expert_of<L>(lane, c * 8);
+            if constexpr (DT == AW4_F32) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (have <= (WHOLE ? 0 : i)) w[i] = kNegInf;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (have <= (WHOLE ? 0 : 2 * i)) w[i] = kNegInf << 16 | kNegInf;
+                    if constexpr (!WHOLE)
+                        if (have == 2 * i + 1) w[i] = __byte_perm(w[i], kNegInf, 0x5410);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void widen(float l[V]) const {
 #pragma unroll
         for (int c = 0; c < V / 8; ++c) widen8<DT>(raw[c], l + c * 8);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (!in || (!WHOLE && expert_of<L>(lane, i) >= experts)) l[i] = -INFINITY;
     }
 };
 
 // One pass over the logits, a row to L lanes, so that selections and sums are shuffles.  Bound by
-// instructions (selections half of them): 65536 x 128 bf16, k = 8, in 27 us, where 10 MB a direction would take 4.
-// Blocks of T threads stay, one an SM, their sums over rows in registers: 1024 threads, or what registers
-// allow from 257 experts on; 256 where 1024 would leave SMs without a row (48 x 8: 4.5 us for 6.5).
+// instructions (sort and selections half of them): 65536 x 128, k = 8, in 22.5 us in bf16 and 34.5 in float32, where
+// the bytes would take 4 and 6.  Blocks of T threads stay, one an SM, their sums over rows in registers: as many
+// threads as registers allow, or 256 where those would leave SMs without a row (48 x 8: 4.5 us for 6.5).
 constexpr int kRouteFew = 256;
 template <int V>
-constexpr int kRouteMost = V == 8 ? 1024 : V == 16 ? 512 : 256;
+constexpr int kRouteMost = V == 8 ? 1024 : V == 16 ? 768 : 512;
 
 // What the blocks of a call add up, zero before it.  The sums of p are whole
 // numbers of 2^-32, so that the order of the additions does not matter; a
@@ -225,25 +230,32 @@ __host__ __device__ constexpr int64_t route_totals_bytes(int experts) {
     return (int64_t)sizeof(RouteTotals) + 12 * (int64_t)experts;
 }
 
+// Words of shared memory in front of a forward block's counts.
+template <int DT, int L, int V, int T>
+__host__ __device__ constexpr int route_work_words(int k) {
+    using P = Picker<DT, L, V>;
+    const int rows = P::kShared * T + T / L * k * ((int)sizeof(typename P::Key) / 4), sums = T / 32 * V * L;
+    return rows > sums ? rows : sums;
+}
+
 template <int DT, int L, int V, bool WHOLE, int T>
-__global__ void __launch_bounds__(T, V == 8 ? 1024 / T : 1)
+__global__ void __launch_bounds__(T, kRouteMost<V> / T)
 route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, const uint8_t* __restrict__ valid,
                      bool renormalize, float* __restrict__ weights, int32_t* __restrict__ chosen,
                      float2* __restrict__ stats, RouteTotals* __restrict__ totals, int32_t* __restrict__ counts,
                      int32_t* __restrict__ valid_rows, float* __restrict__ balance) {
     constexpr int kThreads = T, kRows = kThreads / L;
-    extern __shared__ int32_t smem[];
+    using P = Picker<DT, L, V>;
+    using Key = typename P::Key;
+    // the lists and choices of the rows in work, later the warps' sums, and behind them the counts
+    extern __shared__ __align__(16) uint32_t work[];
     __shared__ float scratch[kThreads / 32];
     __shared__ int is_last;
-    int32_t* count = smem;                                            // [experts + 1], the last: valid rows
-    uint32_t* key_s = reinterpret_cast<uint32_t*>(count + experts + 1);       // [rows][k]
-    int32_t* chosen_s = reinterpret_cast<int32_t*>(key_s + kRows * k);
+    int32_t* count = reinterpret_cast<int32_t*>(work) + route_work_words<DT, L, V, T>(k);      // [experts + 1], the last: valid rows
     for (int i = threadIdx.x; i <= experts; i += kThreads) count[i] = 0;
     __syncthreads();
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
-    uint32_t* my_key = key_s + group * k;
-    int32_t* my_chosen = chosen_s + group * k;
-    uint32_t* sorted_s = reinterpret_cast<uint32_t*>(chosen_s + kRows * k);   // what a Picker keeps
+    Key* my_key = reinterpret_cast<Key*>(work + P::kShared * kThreads) + group * k;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
@@ -262,31 +274,25 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
         const bool in = row < rows;
         bool ok = in && now_valid;
         float l[V];
-        now.widen(l, lane, experts, ok);
+        now.mask(lane, experts, ok);
+        now.widen(l);
+        P picker(now.raw, lane, work, kThreads);
         from += from_step;
         now.load(logits, from, lane, experts, row + step < rows);
         if (valid && row + step < rows) now_valid = valid[row + step];
-        using P = Picker<DT, L, V>;
-        P picker(l, lane, sorted_s, kThreads);
         // The k largest, kept by the lanes in turn: a lane's first in registers, any further ones in shared
         // memory.
-        int at = 0, mine_at = 0;
-        const uint32_t first = picker.next(lane, at);
-        uint32_t mine_key = first;
-        mine_at = at;
+        const Key first = picker.next();
+        Key mine_key = first;
         const int few = min(k, L);
 #pragma unroll 2
         for (int j = 1; j < few; ++j) {
-            const uint32_t best = picker.next(lane, at);
+            const Key best = picker.next();
             mine_key = lane == j ? best : mine_key;
-            if constexpr (DT == AW4_F32) mine_at = lane == j ? at : mine_at;
         }
         for (int j = few; j < k; ++j) {
-            const uint32_t best = picker.next(lane, at);
-            if (lane == j % L) {
-                my_key[j] = best;
-                if constexpr (DT == AW4_F32) my_chosen[j] = at;
-            }
+            const Key best = picker.next();
+            if (lane == j % L) my_key[j] = best;
         }
         ok = ok && P::some(first);
         const float top = P::value(first);
@@ -317,14 +323,14 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
                 if (ok) atomicAdd(&count[experts], 1);
             }
             if (lane < few) {
-                const int e = take ? P::expert(mine_key, mine_at) : -1;
+                const int e = take ? P::expert(mine_key) : -1;
                 weights[picks_at + lane] = mine_w * scale;
                 chosen[picks_at + lane] = e;
                 if (take) atomicAdd(&count[e], 1);
             }
             for (int j = lane + L; j < k; j += L) {
                 const bool more = ok && P::some(my_key[j]);
-                const int e = more ? P::expert(my_key[j], DT == AW4_F32 ? my_chosen[j] : 0) : -1;
+                const int e = more ? P::expert(my_key[j]) : -1;
                 weights[picks_at + j] = more ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
                 chosen[picks_at + j] = e;
                 if (more) atomicAdd(&count[e], 1);
@@ -337,7 +343,7 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
 #pragma unroll
         for (int o = 16; o >= L; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
     __syncthreads();
-    float* warp_sums = reinterpret_cast<float*>(key_s);       // [kThreads / 32][V L]: the choices are out
+    float* warp_sums = reinterpret_cast<float*>(work);       // [kThreads / 32][V L]: the choices are out
     if ((threadIdx.x & 31) < L)
 #pragma unroll
         for (int i = 0; i < V; ++i) warp_sums[(threadIdx.x >> 5) * (V * L) + expert_of<L>(lane, i)] = acc[i];
@@ -453,7 +459,8 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         const int at = now_at;
         const float w = now_w, d = now_d;
         float l[V];
-        now.widen(l, lane, experts, ok);
+        now.mask(lane, experts, ok);
+        now.widen(l);
         from += from_step;
         fetch(row + step, picks_at + k_step);
         // up to L choices a lane has one, the one that came with the logits
@@ -497,7 +504,31 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
     }
 }
 
-// Lanes of a row: the fewest that hold eight logits each, a whole warp from 256 experts on.
+// Lanes of a row in the forward kernel.  Fewer lanes with more logits each make a warp's selections serve more rows (65536
+// rows in bf16: 128 experts by 8 lanes 22.5 us, by 16 26.7, by 4 28.8; 256 by 8 30.5, by 16 35.0, by 32
+// 37.1; 64 by 4 16.6, by 8 18.1), until a row's logits and sums fill the registers; from 257 experts on a whole
+// warp has its maximum in one instruction (16384 x 512: 21 us, by 16 lanes 25).
+constexpr int route_lanes(int experts) {
+    return experts <= 8 ? 1 : experts <= 16 ? 2 : experts <= 64 ? 4 : experts <= 256 ? 8 : 32;
+}
+template <int E, typename F>
+static int32_t route_lanes_shape(F f) {
+    constexpr int kLanes = route_lanes(E);
+    return f(std::integral_constant<int, kLanes>(), std::integral_constant<int, E / kLanes>());
+}
+template <typename F>
+static int32_t route_shape_forward(int experts, F f) {
+    if (experts <= 8) return route_lanes_shape<8>(f);
+    if (experts <= 16) return route_lanes_shape<16>(f);
+    if (experts <= 32) return route_lanes_shape<32>(f);
+    if (experts <= 64) return route_lanes_shape<64>(f);
+    if (experts <= 128) return route_lanes_shape<128>(f);
+    if (experts <= 256) return route_lanes_shape<256>(f);
+    if (experts <= 512) return route_lanes_shape<512>(f);
+    return route_lanes_shape<1024>(f);
+}
+
+// Lanes of a row in the backward kernel: the fewest that hold eight logits each, up to a whole warp.
 template <typename F>
 static int32_t route_shape(int experts, F f) {
     using std::integral_constant;
@@ -519,12 +550,9 @@ static int32_t route_by_dtype(int dtype, F f) {
     return f(integral_constant<int, AW4_F16>());
 }
 
-// The form of a call: WHOLE only up to 256 experts, eight logits a lane.
-template <int V, typename F>
+template <typename F>
 static int32_t route_form(bool whole, F f) {
-    if constexpr (V == 8)
-        if (whole) return f(std::true_type());
-    return f(std::false_type());
+    return whole ? f(std::true_type()) : f(std::false_type());
 }
 
 static int32_t check_route(const char* what, int dtype, int64_t rows, int64_t experts, int32_t k) {
@@ -538,20 +566,19 @@ static int32_t check_route(const char* what, int dtype, int64_t rows, int64_t ex
     return AW4_OK;
 }
 
-static int route_lanes(int experts) {
-    int lanes = 1;
-    while (lanes < 32 && lanes * 8 < experts) lanes *= 2;
-    return lanes;
+static int route_most(int experts) {
+    int values = 8;
+    while (values * route_lanes(experts) < experts) values *= 2;
+    return values == 8 ? kRouteMost<8> : values == 16 ? kRouteMost<16> : kRouteMost<32>;
 }
-
 // Threads of the forward kernel's blocks, and blocks: as many as have a row, at most one an SM (of 256 threads four).
 static int route_threads(int device, int64_t rows, int experts) {
-    const int most = experts <= 256 ? kRouteMost<8> : experts <= 512 ? kRouteMost<16> : kRouteMost<32>;
+    const int most = route_most(experts);
     return rows * route_lanes(experts) / most < sm_count(device) ? kRouteFew : most;
 }
 static int route_grid(int device, int64_t rows, int experts) {
     const int threads = route_threads(device, rows, experts), per = threads / route_lanes(experts);
-    const int64_t resident = (int64_t)sm_count(device) * (threads == kRouteFew && experts <= 256 ? 4 : 1);
+    const int64_t resident = (int64_t)sm_count(device) * (threads == kRouteFew ? route_most(experts) / kRouteFew : 1);
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, resident));
 }
 
@@ -596,18 +623,14 @@ extern "C" int32_t aw4_route_forward(const void* logits, int32_t dtype, int64_t 
         if (e != cudaSuccess) return fail(AW4_ERR_CUDA, "route_forward: %s", cudaGetErrorString(e));
     }
     return route_by_dtype(dtype, [&](auto dt) {
-        return route_shape(experts, [&](auto lanes, auto v) {
+        return route_shape_forward(experts, [&](auto lanes, auto v) {
             const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
             const bool all_whole = rows_whole(logits, ld, experts, dtype) && experts == lanes.value * v.value;
-            return route_form<v.value>(all_whole, [&](auto whole) {
+            return route_form(all_whole, [&](auto whole) {
                 auto go = [&](auto threads) -> int32_t {
                     constexpr int kThreads = threads.value;
-                    // choices of the rows in work, later the warps' sums
-                    const int choices = std::max(2 * (kThreads / lanes.value) * k +
-                                                     Picker<dt.value, lanes.value, v.value>::kShared * kThreads,
-                                                 kThreads / 32 * v.value * lanes.value);
                     auto kernel = route_forward_kernel<dt.value, lanes.value, v.value, whole.value, kThreads>;
-                    const int bytes = (experts + 1 + choices) * 4;
+                    const int bytes = (route_work_words<dt.value, lanes.value, v.value, kThreads>(k) + experts + 1) * 4;
                     if (bytes > 40 * 1024) {
                         const cudaError_t e =
                             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -648,7 +671,7 @@ extern "C" int32_t aw4_route_backward(const void* logits, int32_t dtype, int64_t
                                                    (int64_t)sm_count(device) * kRouteBackBlocks<v.value>);
             const RowsIn in = route_rows(logits, rows, experts, ld, dtype);
             const RowsOut out = {static_cast<char*>(dlogits), experts, rows_on(dlogits, experts, dtype, 16)};
-            return route_form<v.value>(rows_whole(logits, ld, experts, dtype) && rows_whole(dlogits, experts, experts, dtype) &&
+            return route_form(rows_whole(logits, ld, experts, dtype) && rows_whole(dlogits, experts, experts, dtype) &&
                                            experts == lanes.value * v.value, [&](auto whole) {
             route_backward_kernel<dt.value, lanes.value, v.value, whole.value>
                 <<<grid, kRouteBackThreads, 0, (cudaStream_t)stream>>>(

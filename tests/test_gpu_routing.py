@@ -235,3 +235,44 @@ def test_gradient_of_a_missing_choice_is_ignored():
         r = Q.route_forward(logits.to(DEV), 3, renormalize=renormalize)
         dl = Q.route_backward(dw.to(DEV), None, r)
         assert r.experts[2].tolist() == [0, -1, -1] and torch.isfinite(dl).all()
+
+
+@pytest.mark.parametrize("experts", [8, 16, 32, 64, 100, 128, 256, 512, 1024])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=_ids)
+def test_order_of_every_16_bit_pattern(dtype, experts):
+    # both zeros, every payload and sign of a NaN, infinities and subnormal numbers
+    g = torch.Generator().manual_seed(experts)
+    bits = torch.randperm(65536, generator=g)[: 65536 // experts * experts]
+    logits = (bits - 32768).to(torch.int16).view(dtype).view(-1, experts)
+    k = min(experts, 32)
+    order = logits.double()
+    order[order == math.inf] = 1e300
+    order[order.isnan()] = math.inf
+    order, want = order.sort(dim=-1, descending=True, stable=True)
+    want[order == -math.inf] = -1
+    got = Q.route_forward(logits.to(DEV), k).experts.cpu()
+    assert torch.equal(got.long(), want[:, :k])
+
+
+@pytest.mark.parametrize("experts,k", [(64, 8), (128, 10), (200, 12), (256, 32), (512, 3)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+def test_more_rows_than_the_blocks_hold(dtype, experts, k):
+    # the wide blocks, several rounds of rows in each; choices against a sort, counts against the choices
+    rows = 40009
+    logits = torch.randn(rows, experts, generator=torch.Generator(DEV).manual_seed(k), device=DEV).to(dtype)
+    valid = torch.ones(rows, dtype=torch.bool, device=DEV)
+    valid[5::7] = False
+    r = Q.route_forward(logits, k, valid=valid)
+    want = logits.double().sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    want[5::7] = -1
+    assert torch.equal(r.experts.long(), want)
+    assert torch.equal(r.counts.long(), torch.bincount(want[want >= 0], minlength=experts))
+    p = torch.softmax(logits.double(), -1)
+    w = p.gather(-1, want.clamp(min=0))
+    w = torch.where(want >= 0, w / w.sum(-1, keepdim=True), 0.0)
+    # a probability is (2 (4 + |l - max|) + experts) 2^-24 off, as above; |l| < 8
+    one = (2 * (4 + 16) + experts) * EPS32
+    assert ((r.weights.double() - w).abs() <= 2 * one * w).all()
+    n = valid.sum().double()
+    balance = (experts * r.counts.double() / (k * n) * p[valid].sum(0) / n).sum().item()
+    assert abs(r.balance_loss.item() - balance) <= (one + (rows + experts + 8) * EPS32) * balance
