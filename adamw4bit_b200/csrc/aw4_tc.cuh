@@ -25,8 +25,14 @@ __device__ __forceinline__ uint32_t in_first_block(uint32_t bar) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
     return r;
 }
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+// Arrivals there.  An arrival that names no scope orders memory within its own block only.  `release`: what this
+// thread has written, or has seen written by a wait, is there for the thread whose wait of kind kWaitPair sees the arrival.
+// `relaxed`: no memory is handed over; tensor memory is ordered by the tcgen05 fences around arrival and wait.
+__device__ __forceinline__ void bar_arrive_pair_release(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_pair_relaxed(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ uint32_t block_in_pair() {
     uint32_t r;
@@ -39,11 +45,24 @@ __device__ __forceinline__ void pair_sync() {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Whose arrivals a wait is for: the own block's threads and copies and the tensor core's commits, or
+// the other block's threads too, by either kind of arrival.
+enum WaitKind { kWaitOwn, kWaitPair, kWaitPairRelaxed };
+template <WaitKind KIND = kWaitOwn>
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if constexpr (KIND == kWaitPair)
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else if constexpr (KIND == kWaitPairRelaxed)
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ uint64_t now_ns() {
@@ -57,10 +76,11 @@ __device__ __forceinline__ uint64_t now_ns() {
 // down.
 constexpr int kWaitTries = 1 << 24;
 constexpr uint64_t kWaitNs = 2000000000ull;
+template <WaitKind KIND = kWaitOwn>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     uint64_t from = 0;
     for (int i = 0; i < kWaitTries; ++i) {
-        if (bar_try(bar, parity)) return true;
+        if (bar_try<KIND>(bar, parity)) return true;
         if ((i & 63) == 63) {
             if (*gave_up) return false;
             const uint64_t t = now_ns();

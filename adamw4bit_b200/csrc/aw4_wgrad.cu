@@ -13,7 +13,13 @@
 //                of warps taking turns.  A lane owns a block of 32 codes of one row
 //   warp 17      (first block) tcgen05.mma for the pair, both operands with the row
 //                index as the inner dimension
+//   warps 18-19  (second block) tell the first that a group's values are there
 //   warps 0-15   accumulators -> dW, or a float32 partial tile
+//
+// The values of the second block are written by its threads and read for a product that the first
+// block issues: its arrivals release, and the wait for them acquires, over the pair.  A warp of its own for each group's
+// arrivals keeps that release (some hundred cycles) out of the conversion: 8192 x 14336 x 4096 in 734 us, 751 with one such warp
+// for both groups, 770 with an arrival of every converting warp.
 //
 // A pair, because shared memory bounds a single block: for 256 x 256 x 64 its tensor
 // core reads 96 KB of operands, and copies and conversion move 96 KB more, 1536
@@ -26,9 +32,8 @@
 // Rows behind a group's last are zeroed in both operands (a NaN of the next
 // group must not meet a zero).
 //
-// Bound by the tensor cores at the power limit: 8192 x 14336 x 4096 bf16 in 690 us, 1396 TFLOP/s (cuBLAS on bf16
-// values 631 us on the same chip; 798 and 725 us in a loop of seconds, where both clock down).  A step of 64 rows
-// takes 0.78 us for 1024 cycles of products; conversion and copies alone 0.52.
+// Bound by the tensor cores at the power limit and by the way from values to product: 8192 x 14336 x 4096 bf16 in 734 us,
+// 1311 TFLOP/s (cuBLAS on bf16 values 631 us).  A step of 64 rows takes 0.83 us for 1024 cycles of products.
 //
 // Work split: whole tiles go round the pairs, n-tiles outermost so that
 // pairs that run together share dy and codes in L2; the last wave and what
@@ -53,8 +58,8 @@ constexpr int kWgTileN = 512, kWgTileK = 256;   // a pair's tile
 constexpr int kWgRows = 64;                     // rows of a step
 constexpr int kWgStages = 4, kWgBuffers = 4;    // even: see the converting warps
 constexpr int kWgConvert = 512;                 // threads that convert and write out, in two groups
-constexpr int kWgThreads = kWgConvert + 64;
-constexpr int kWgCopy = kWgConvert / 32, kWgProduct = kWgCopy + 1;   // warps
+constexpr int kWgThreads = kWgConvert + 128;
+constexpr int kWgCopy = kWgConvert / 32, kWgProduct = kWgCopy + 1, kWgTell = kWgProduct + 1;   // warps
 constexpr int kWgBox = kWgRows * 128;           // a copied box: 64 lines of 128 bytes
 constexpr int kWgDyBytes = 4 * kWgBox;          // a block's 2 x 128 columns of dy
 constexpr int kWgCodeBytes = kWgBox;            // its 128 codes of each row
@@ -376,7 +381,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
             bar_init(smem_addr(&s.empty[i]), 1);
         }
         for (int i = 0; i < kWgBuffers; ++i) {
-            bar_init(smem_addr(&s.ready[i]), kWgConvert / 32);   // one group of each block
+            bar_init(smem_addr(&s.ready[i]), kWgConvert / 64 + (side == 0));   // a group; the second block's word
             bar_init(smem_addr(&s.done[i]), 1);
         }
         bar_init(smem_addr(&s.acc_full), 1);
@@ -445,11 +450,11 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 const WgTile t = wg_tile(p, seg.tile);
                 const uint32_t idesc = tc_idesc(DT == AW4_BF16, 2 * t.half);
                 const bool two = t.n0 + 256 < p.n;
-                ok = bar_wait(smem_addr(&s.acc_empty), (i & 1) ^ 1, gave_up);
+                ok = bar_wait<kWaitPairRelaxed>(smem_addr(&s.acc_empty), (i & 1) ^ 1, gave_up);
                 for (int step = seg.first; ok && step < seg.last; ++step, ++c) {
                     const int st = c % kWgStages;
                     ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
-                         bar_wait(smem_addr(&s.ready[buf]), turn, gave_up);
+                         bar_wait<kWaitPair>(smem_addr(&s.ready[buf]), turn, gave_up);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t dy_a = smem_addr(dy_s + st * kWgDyBytes);
@@ -473,6 +478,27 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
             if (!ok) {   // products in flight end before the tensor memory goes
                 tc_commit(smem_addr(&s.drain));
                 bar_drain(smem_addr(&s.drain), 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= kWgTell) {
+        if (lane == 0 && side == 1) {
+            const uint32_t group = warp - kWgTell;
+            uint32_t c = 0, buf = 0, turn = 0;
+            bool ok = true;
+            for (int i = 0; ok && i < segments; ++i) {
+                const WgSegment seg = wg_segment(p, s, i, pair, pairs);
+                for (int step = seg.first; step < seg.last; ++step, ++c) {
+                    if ((c & 1) == group) {
+                        ok = bar_wait(smem_addr(&s.ready[buf]), turn, gave_up);
+                        if (!ok) break;
+                        bar_arrive_pair_release(in_first_block(smem_addr(&s.ready[buf])));
+                    }
+                    if (++buf == kWgBuffers) {
+                        buf = 0;
+                        turn ^= 1;
+                    }
+                }
             }
         }
         __syncwarp();
@@ -520,7 +546,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                     byte = next;
                     fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(in_first_block(smem_addr(&s.ready[buf])));
+                    if (lane == 0) bar_arrive(smem_addr(&s.ready[buf]));
                 }
                 if (++buf == kWgBuffers) {
                     buf = 0;
@@ -569,7 +595,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
             __syncwarp();
             if (lane == 0) {
                 bar_arrive(smem_addr(&s.out_done));
-                bar_arrive_cluster(in_first_block(smem_addr(&s.acc_empty)));
+                bar_arrive_pair_relaxed(in_first_block(smem_addr(&s.acc_empty)));
             }
         }
     }
