@@ -147,18 +147,38 @@ def check(rc: int, what: str) -> None:
         raise NativeError(f"{what}: {kind}: {msg}")
 
 
-_wait_status: torch.Tensor | None = None
+# One pinned word a device, kept for the process: a kernel sets it when one of its waits runs out.
+_wait_words: dict[int, torch.Tensor] = {}
 
 
-def wait_status() -> int:
-    """Address of the pinned word that a kernel sets when one of its waits runs out.  It is looked at before
-    each launch that passes it: the outputs of the launch that set it are not to be used."""
-    global _wait_status
-    if _wait_status is None:
-        _wait_status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-    elif ctypes.c_int32.from_address(_wait_status.data_ptr()).value:
-        raise NativeError("a kernel of an earlier call gave up a wait; its outputs are not complete")
-    return _wait_status.data_ptr()
+def _new_wait_word() -> torch.Tensor:
+    return torch.zeros(1, dtype=torch.int32, pin_memory=True)
+
+
+def raise_given_up(device: int | None = None) -> None:
+    """Raises, once, where a kernel of a device (of any) that has run so far gave up a wait."""
+    for index in list(_wait_words) if device is None else (device,):
+        word = _wait_words.get(index)
+        if word is None:
+            continue
+        flag = ctypes.c_int32.from_address(word.data_ptr())
+        if flag.value:
+            flag.value = 0
+            raise NativeError(f"cuda:{index}: a weight gradient gave up a wait, its result is not complete")
+
+
+def wait_status(device: int) -> int:
+    """Address of the word that the device's next launch sets when one of its waits runs out.  Raises for an
+    earlier launch that did."""
+    word = _wait_words.get(device)
+    if word is None:
+        with _lock:                     # backward passes run on a thread for each device
+            word = _wait_words.get(device)
+            if word is None:
+                word = _wait_words[device] = _new_wait_word()
+    else:
+        raise_given_up(device)
+    return word.data_ptr()
 
 
 def launch_count() -> int:

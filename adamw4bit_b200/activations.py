@@ -38,7 +38,7 @@ from . import _native as N
 __all__ = [
     "Act8", "RMSNormSaved", "SwiGLUSaved", "quantize_act8", "dequantize_act8", "rms_norm",
     "rms_norm_forward", "rms_norm_backward", "swiglu", "swiglu_forward", "swiglu_backward", "linear",
-    "grouped_linear", "weight_grad",
+    "grouped_linear", "weight_grad", "check_weight_grads",
 ]
 
 BLOCK = 32
@@ -425,8 +425,24 @@ def weight_grad(dy: torch.Tensor, x8: Act8, offsets: torch.Tensor | None = None,
     ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     N.check(N.lib().aw4_weight_grad(src.data_ptr(), N.DTYPE_CODES[dy.dtype], rows, n, ld, *_ptrs(x8), k,
                                     N.ptr(offsets), groups, out.data_ptr(), N.DTYPE_CODES[out.dtype],
-                                    int(accumulate), N.ptr(ws), nbytes, N.wait_status(), dev, N.stream_of(dev)), "aw4_weight_grad")
+                                    int(accumulate), N.ptr(ws), nbytes, N.wait_status(dev), dev, N.stream_of(dev)),
+            "aw4_weight_grad")
     return out
+
+
+def check_weight_grads(device: torch.device | int | str | None = None, *, synchronize: bool = True) -> None:
+    """Raises ``NativeError`` where a weight gradient on this device (the current one) gave up a wait, and forgets
+    it.  ``synchronize`` first waits for the device; without it only what has run so far is seen.  The next
+    ``weight_grad`` on the device and an optimizer's ``step`` look too, without waiting: a program that uses gradients
+    elsewhere, or replays them from a CUDA graph, calls this before it relies on them."""
+    if isinstance(device, str):
+        device = torch.device(device)
+    index = device if isinstance(device, int) else device.index if device is not None else None
+    if index is None:
+        index = torch.cuda.current_device()
+    if synchronize:
+        torch.cuda.synchronize(index)
+    N.raise_given_up(index)
 
 
 def _check_linear(x: torch.Tensor, weight: torch.Tensor, x8: Act8 | None, what: str) -> None:

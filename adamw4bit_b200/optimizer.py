@@ -417,6 +417,7 @@ class QuantizedAdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        N.raise_given_up()              # a gradient that is known not to be complete is not stepped with
         plan = _StepPlan(self)
         ordinal = 0
         for group in self.param_groups:

@@ -340,6 +340,7 @@ class ZeRO1AdamW4Bit:
             raise RuntimeError('grad_reduce="multicast": a parameter\'s .grad is no longer '
                                'the bound view; zero gradients with the optimizer\'s '
                                'zero_grad(), not by setting them to None')
+        N.raise_given_up()              # a gradient that is known not to be complete is not stepped with
         self.step_count += 1
         t = self.step_count
         hy = hyper_scalars(self.lr, self.betas[0], self.betas[1], self.eps, self.wd, t,
