@@ -108,6 +108,7 @@ SIGNATURES = {
     "aw4_rms_norm_backward_workspace": ([_I64, _I64, _I32], _U64),
     "aw4_rms_norm_backward": ([_VP, _I32, _I64, _I64, _I64, *[_VP] * 4, _I32, _VP, _VP, _VP, _I64, _I32,
                                _VP], _I32),
+    "aw4_set_wait_limit": ([_U64], _I32),
     "aw4_weight_grad_workspace": ([_I64, _I64, _I64, _I64, _I32], _U64),
     "aw4_weight_grad": ([_VP, _I32, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _VP, _I32, _I32, _VP, _I64,
                          _VP, _I32, _VP], _I32),

@@ -71,21 +71,21 @@ __device__ __forceinline__ uint64_t now_ns() {
     return t;
 }
 // Waits for the phase of this parity to end.  Every wait has a limit in tries
-// and in time, far above the longest tile: past it, or once another waiter of
+// and in time (`limit`, in ns), by default far above the longest tile: past it, or once another waiter of
 // the block has given up (`gave_up`), it returns false and the block winds
-// down.
+// down.  With a limit of 0 it returns false at once.
 constexpr int kWaitTries = 1 << 24;
 constexpr uint64_t kWaitNs = 2000000000ull;
 template <WaitKind KIND = kWaitOwn>
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, uint64_t limit) {
     uint64_t from = 0;
-    for (int i = 0; i < kWaitTries; ++i) {
+    for (int i = 0; limit && i < kWaitTries; ++i) {
         if (bar_try<KIND>(bar, parity)) return true;
         if ((i & 63) == 63) {
             if (*gave_up) return false;
             const uint64_t t = now_ns();
             if (!from) from = t;
-            if (t - from > kWaitNs) break;
+            if (t - from > limit) break;
         }
     }
     *gave_up = 1;

@@ -45,6 +45,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/adamw4bit_b200.h"
@@ -92,6 +93,7 @@ struct WgParams {
     float* partial;
     WgSlot* slots;              // null: no tile is cut
     int32_t* status;
+    uint64_t wait_ns;           // limit of a wait
 };
 
 struct WgShared {
@@ -361,6 +363,26 @@ __device__ __forceinline__ float4* wg_partial(const WgParams& p, int slot, int r
     return reinterpret_cast<float4*>(p.partial) + ((int64_t)slot * (kWgTileK / 4) + col / 4) * kWgTileN + row;
 }
 
+// Of a converting warp that has given up a wait before tile `from`: NaN in its place of that and of the tiles behind
+// it, so that what is missing shows in the result, which a replayed graph or a program that does not look at the status
+// may use.  Not through shared memory, where products in flight may read.
+template <int OT>
+__device__ __noinline__ void wg_no_numbers(const WgParams& p, const WgShared& s, int from, int pair, int pairs, int side) {
+    const float nan = __uint_as_float(0x7fc00000u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row_in = ((warp >> 2) & 1) * 256 + side * 128 + (warp & 3) * 32 + lane;
+    for (int i = from; i < s.whole + s.cuts; ++i) {
+        const WgSegment seg = wg_segment(p, s, i, pair, pairs);
+        const WgTile t = wg_tile(p, seg.tile);
+        const int n = t.n0 + row_in, end = min((warp >> 3) * 128 + 128, p.k - t.k0);
+        if (n >= p.n) continue;
+        for (int col = (warp >> 3) * 128; col < end; ++col) {
+            if (seg.slot < 0) Elem<OT>::store1(p.out, ((int64_t)t.g * p.n + n) * p.k + t.k0 + col, nan);
+            else if (col % 4 == 0) *wg_partial(p, seg.slot, row_in, col) = make_float4(nan, nan, nan, nan);
+        }
+    }
+}
+
 template <int DT, int OT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
 weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_constant__ CUtensorMap code_map,
@@ -423,7 +445,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 bytes += codes_in ? kWgBox : 0;
                 for (int step = seg.first; step < seg.last; ++step, ++c) {
                     const int st = c % kWgStages;
-                    ok = bar_wait(smem_addr(&s.empty[st]), ((c / kWgStages) & 1) ^ 1, gave_up);
+                    ok = bar_wait(smem_addr(&s.empty[st]), ((c / kWgStages) & 1) ^ 1, gave_up, p.wait_ns);
                     if (!ok) break;
                     const uint32_t bar = smem_addr(&s.full[st]);
                     const int row = (int)(t.first + (int64_t)step * kWgRows);
@@ -450,11 +472,11 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 const WgTile t = wg_tile(p, seg.tile);
                 const uint32_t idesc = tc_idesc(DT == AW4_BF16, 2 * t.half);
                 const bool two = t.n0 + 256 < p.n;
-                ok = bar_wait<kWaitPairRelaxed>(smem_addr(&s.acc_empty), (i & 1) ^ 1, gave_up);
+                ok = bar_wait<kWaitPairRelaxed>(smem_addr(&s.acc_empty), (i & 1) ^ 1, gave_up, p.wait_ns);
                 for (int step = seg.first; ok && step < seg.last; ++step, ++c) {
                     const int st = c % kWgStages;
-                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
-                         bar_wait<kWaitPair>(smem_addr(&s.ready[buf]), turn, gave_up);
+                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up, p.wait_ns) &&
+                         bar_wait<kWaitPair>(smem_addr(&s.ready[buf]), turn, gave_up, p.wait_ns);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t dy_a = smem_addr(dy_s + st * kWgDyBytes);
@@ -490,7 +512,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 const WgSegment seg = wg_segment(p, s, i, pair, pairs);
                 for (int step = seg.first; step < seg.last; ++step, ++c) {
                     if ((c & 1) == group) {
-                        ok = bar_wait(smem_addr(&s.ready[buf]), turn, gave_up);
+                        ok = bar_wait(smem_addr(&s.ready[buf]), turn, gave_up, p.wait_ns);
                         if (!ok) break;
                         bar_arrive_pair_release(in_first_block(smem_addr(&s.ready[buf])));
                     }
@@ -509,7 +531,8 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
         const int r = (warp & 7) * 8 + (lane >> 2), j = lane & 3;
         uint32_t c = 0, buf = 0, turn = 0;
         bool ok = true;
-        for (int i = 0; ok && i < segments; ++i) {
+        int i = 0;
+        for (; i < segments; ++i) {
             const WgSegment seg = wg_segment(p, s, i, pair, pairs);
             const WgTile t = wg_tile(p, seg.tile);
             const uint32_t block = (t.k0 + side * t.half) / kA8Block + j;
@@ -521,7 +544,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
             const uint8_t* scale = p.scales + row * p.blocks + block;
             int byte = cols && row < end ? *scale : 1;
             // the values' buffers also turn the last tile's sums on their way out
-            if (i > 0) ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.out_done), (i - 1) & 1, gave_up));
+            if (i > 0) ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.out_done), (i - 1) & 1, gave_up, p.wait_ns));
             if (!ok) break;
             for (int step = seg.first; step < seg.last; ++step, ++c) {
                 if ((c & 1) == group) {
@@ -530,8 +553,8 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                     row += 2 * kWgRows;
                     scale += 2 * kWgRows * p.blocks;
                     const int next = cols && row < end ? *scale : 1;
-                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up) &&
-                         bar_wait(smem_addr(&s.done[buf]), turn ^ 1, gave_up);
+                    ok = bar_wait(smem_addr(&s.full[st]), (c / kWgStages) & 1, gave_up, p.wait_ns) &&
+                         bar_wait(smem_addr(&s.done[buf]), turn ^ 1, gave_up, p.wait_ns);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (cols)
@@ -554,7 +577,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 }
             }
             if (!ok) break;
-            ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.acc_full), i & 1, gave_up));
+            ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&s.acc_full), i & 1, gave_up, p.wait_ns));
             if (!ok) break;
             tc_fence_after();
             // four warps for the 128 rows that this block has of each accumulator; the groups
@@ -598,6 +621,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
                 bar_arrive_pair_relaxed(in_first_block(smem_addr(&s.acc_empty)));
             }
         }
+        if (!ok) wg_no_numbers<OT>(p, s, i, pair, pairs, side);
     }
     // neither block leaves while the other's products or arrivals may reach it
     tc_fence_before();
@@ -667,6 +691,8 @@ weight_grad_join_kernel(const WgParams p, int pairs) {
 // host side
 // ---------------------------------------------------------------------------
 
+static std::atomic<uint64_t> g_wait_ns{kWaitNs};
+
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -731,6 +757,11 @@ static uint64_t wg_workspace(const WgPlan& plan) {
 
 using namespace aw4;
 
+extern "C" int32_t aw4_set_wait_limit(uint64_t ns) {
+    g_wait_ns.store(std::min(ns, kWaitNs), std::memory_order_relaxed);
+    return AW4_OK;
+}
+
 extern "C" uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device) {
     if (rows <= 0 || n <= 0 || k <= 0 || groups < 1) return 0;
     return wg_workspace(wg_plan(device, rows, n, k, groups));
@@ -786,6 +817,7 @@ extern "C" int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, 
     p.partial = static_cast<float*>(workspace);
     p.slots = plan.cuts ? reinterpret_cast<WgSlot*>(p.partial + (int64_t)pairs * 2 * kWgTileN * kWgTileK) : nullptr;
     p.status = status;
+    p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     CUtensorMap dy_map, code_map;
     if (!encode_rows(&dy_map, dtype == AW4_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                      dy, n, rows, ld * 2) ||

@@ -258,7 +258,10 @@ int32_t aw4_rms_norm_backward(const void* dy, int32_t dtype, int64_t rows, int64
  * f16; out_dtype the same or f32.  dy 16-byte aligned, ld at least n and a
  * multiple of 8; workspace 16-byte aligned, contents free.  status: NULL, or a
  * word the device can write (pinned host memory) that the kernel sets to 1
- * when a wait inside it ran out and out is not complete. */
+ * when a wait inside it ran out; what it then has not written of out is NaN.
+ * aw4_set_wait_limit: the limit of such a wait for the launches to come, in
+ * nanoseconds (2 s at first, and at most); 0 gives every wait up at once. */
+int32_t aw4_set_wait_limit(uint64_t ns);
 uint64_t aw4_weight_grad_workspace(int64_t rows, int64_t n, int64_t k, int64_t groups, int32_t device);
 int32_t aw4_weight_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ld,
                         const uint8_t* codes, const uint8_t* scales, int64_t k, const int32_t* offsets,
