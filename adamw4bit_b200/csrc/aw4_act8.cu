@@ -483,7 +483,8 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
         }
         float d0, d1;
         upk2(dot2, d0, d1);
-        const float k = r * r * r * (row_sum<NT>(d0 + d1, part, slot) * inv_cols);
+        // r by r: r^3 alone is beyond float32's normal numbers where r is beyond 2^-42 or 2^42
+        const float k = r * (r * (r * (row_sum<NT>(d0 + d1, part, slot) * inv_cols)));
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int u = j * NT + t;
