@@ -56,12 +56,20 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return v;
 }
 
-// exp(l - top): 2^-22 of the value, and 2^-24 |l - top| of it.  The difference comes
-// first: products of logits near the type's limits would overflow.
+// exp(l - top).  The difference comes first: products of logits near the type's limits would overflow.
+// FULL: to the last bit or two of float32, for float32 logits and for the weights, which are float32 whatever the logits are.
+// Else the hardware's exponential, 2^-22 of the value and 1.25 * 2^-24 |l - top| of it, in the sums and 16-bit gradients of 16-bit
+// logits: in a sum the terms far from the top are small, and a gradient's rounding is coarser.  65536 x 128 float32, k = 8: forward
+// 34.9 us and backward 18.5 in full, 33.7 and 14.5 with the hardware's.
+template <bool FULL>
 __device__ __forceinline__ float exp_from(float l, float top) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((l - top) * 1.44269504f));
-    return r;
+    if constexpr (FULL) {
+        return expf(l - top);
+    } else {
+        float r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((l - top) * 1.44269504f));
+        return r;
+    }
 }
 
 // Sorts eight words, the largest first (Batcher's odd-even merge).
@@ -299,7 +307,7 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
         float part = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = exp_from(l[i], top);
+            l[i] = exp_from<DT == AW4_F32>(l[i], top);
             part += l[i];
         }
         const float total = lanes_sum<L>(part);
@@ -308,12 +316,12 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(l[i], inv, acc[i]);
         const bool take = ok && lane < few && P::some(mine_key);
-        const float mine_w = take ? exp_from(P::value(mine_key), top) : 0.0f;
+        const float mine_w = take ? exp_from<true>(P::value(mine_key), top) : 0.0f;
         float scale = inv;
         if (renormalize) {
             float chosen_sum = mine_w;
             for (int j = lane + L; j < k; j += L)
-                if (ok && P::some(my_key[j])) chosen_sum += exp_from(P::value(my_key[j]), top);
+                if (ok && P::some(my_key[j])) chosen_sum += exp_from<true>(P::value(my_key[j]), top);
             chosen_sum = lanes_sum<L>(chosen_sum);
             scale = ok ? 1.0f / chosen_sum : 0.0f;
         }
@@ -331,7 +339,7 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
             for (int j = lane + L; j < k; j += L) {
                 const bool more = ok && P::some(my_key[j]);
                 const int e = more ? P::expert(my_key[j]) : -1;
-                weights[picks_at + j] = more ? exp_from(P::value(my_key[j]), top) * scale : 0.0f;
+                weights[picks_at + j] = more ? exp_from<true>(P::value(my_key[j]), top) * scale : 0.0f;
                 chosen[picks_at + j] = e;
                 if (more) atomicAdd(&count[e], 1);
             }
@@ -480,7 +488,7 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = ok ? exp_from(l[i], st.x) * st.y : 0.0f;
+            l[i] = ok ? exp_from<DT == AW4_F32>(l[i], st.x) * st.y : 0.0f;
             sum = __fmaf_rn(l[i], share[i], sum);
         }
         sum = lanes_sum<L>(sum);
