@@ -489,11 +489,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets, x8):
+        # cut to the rows, as the weight gradient's kernel cuts them
+        ctx.bounds = [min(max(o, 0), x.shape[0]) for o in offsets.tolist()]
+        if any(b < a for a, b in zip(ctx.bounds, ctx.bounds[1:])):
+            raise ValueError("grouped_linear: offsets that ascend expected: a row belongs to one group")
         if x8 is None and ctx.needs_input_grad[1]:
             x8 = quantize_act8(x)
         ctx.save_for_backward(weight, offsets, x8.data if ctx.needs_input_grad[1] else None)
         ctx.x8 = (x.shape, x.dtype, x8.start if x8 is not None else 0)
-        ctx.bounds = offsets.tolist()
         y = x.new_zeros(x.shape[0], weight.shape[1])
         for g, (a, b) in enumerate(zip(ctx.bounds, ctx.bounds[1:])):
             if b > a:
@@ -518,7 +521,8 @@ class _GroupedLinear(torch.autograd.Function):
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *,
                    x8: Act8 | None = None) -> torch.Tensor:
     """Differentiable x_g W_g^T over groups of rows: x [rows, k], weight [groups, n, k], offsets int32
-    [groups + 1] on the device, ascending from 0 to rows.  Keeps 8 bits of x; all groups' weight
+    [groups + 1] on the device, ascending from 0 to rows (values outside the rows are cut to them; a row of no
+    group gives zeros).  Keeps 8 bits of x; all groups' weight
     gradients are one launch.  The products of the forward pass and of dx are one library product a
     group, for which the offsets are read once on the host (a synchronisation)."""
     _check_linear(x, weight, x8, "grouped_linear")
