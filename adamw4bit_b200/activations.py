@@ -489,6 +489,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets, x8):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("grouped_linear: reads its offsets on the host, which a CUDA graph cannot capture")
         # cut to the rows, as the weight gradient's kernel cuts them
         ctx.bounds = [min(max(o, 0), x.shape[0]) for o in offsets.tolist()]
         if any(b < a for a, b in zip(ctx.bounds, ctx.bounds[1:])):
@@ -524,7 +526,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     [groups + 1] on the device, ascending from 0 to rows (values outside the rows are cut to them; a row of no
     group gives zeros).  Keeps 8 bits of x; all groups' weight
     gradients are one launch.  The products of the forward pass and of dx are one library product a
-    group, for which the offsets are read once on the host (a synchronisation)."""
+    group, for which the offsets are read once on the host (a synchronisation; a CUDA graph cannot capture it)."""
     _check_linear(x, weight, x8, "grouped_linear")
     if x.dim() != 2 or weight.dim() != 3:
         raise ValueError(f"grouped_linear: x [rows, k] and weight [groups, n, k] expected, found "
