@@ -470,12 +470,7 @@ rms_norm_backward_kernel(const RowsIn dy, int64_t rows, int cols, float inv_cols
             float d[8], v[8], wv[8];
             widen8<DT>(now.dy[j], d);
             a8_decode8(now.q[j], a8_scale(now.b[j]), v);
-            vmul8(d, d, v);
-            // behind the last column codes and gradients are zero, but a block may be NaN
-            if (!WHOLE && (j * NT + t) * 8 + 8 > cols)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if ((j * NT + t) * 8 + i >= cols) d[i] = 0.0f;
+            vmul8(d, d, v);             // behind the last column 0, or NaN in a block that has made the row's NaN anyway
             weight8(weight_s, kChunks8, j * NT + t, wv);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) dot2 = f2_fma(pk2(d[i], d[i + 1]), pk2(wv[i], wv[i + 1]), dot2);
