@@ -45,8 +45,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 template <int L>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    // a whole warp's in one instruction (16384 x 1024, k = 8: 74 us by shuffles, 67); that of half a
-    // warp takes longer so (65536 x 128 by 16 lanes: 28.7 us, 30.8)
+    // a whole warp's in one instruction (16384 x 1024 bf16, k = 8: 35.2 us by shuffles, 31.8)
     if constexpr (L == 32) {
         v = __reduce_max_sync(0xffffffffu, v);
     } else {
@@ -217,9 +216,11 @@ struct RowLogits {
 };
 
 // One pass over the logits, a row to L lanes, so that selections and sums are shuffles.  Bound by
-// instructions (sort and selections half of them): 65536 x 128, k = 8, in 22.5 us in bf16 and 34.5 in float32, where
-// the bytes would take 4 and 6.  Blocks of T threads stay, one an SM, their sums over rows in registers: as many
-// threads as registers allow, or 256 where those would leave SMs without a row (48 x 8: 4.5 us for 6.5).
+// instructions (sort and selections half of them): 65536 x 128, k = 8, in 20 us in bf16 (22.6 a call with the clearing of
+// the totals) and 34.9 in float32, where the bytes would take 4 and 6.  Blocks of T threads stay, their sums over rows in
+// registers: one an SM with as many threads as registers allow, or two to four of 256 where those would leave SMs without a
+// row (48 x 8: 4.5 us for 6.5).  Float32 from 33 experts on spills: 28 to 100 bytes a thread up to 128, 160 to 188 up to
+// 256, 4 to 12 up to 512, 40 to 84 above (65536 x 256, k = 8, in 57 us).
 constexpr int kRouteFew = 256;
 template <int V>
 constexpr int kRouteMost = V == 8 ? 1024 : V == 16 ? 768 : 512;
@@ -403,8 +404,9 @@ route_forward_kernel(const RowsIn logits, int64_t rows, int experts, int k, cons
     }
 }
 
-// One pass: logits, statistics and choices in, the gradient out.  65536 x 128 bf16, k = 8, in 15 us; instructions,
-// then HBM (5 us).
+// One pass: logits, statistics and choices in, the gradient out.  65536 x 128 bf16, k = 8, in 14 us (float32 18.5);
+// instructions, then HBM (5 us).  Rows that are not whole vectors spill 28 to 44 bytes a thread at 64 registers, float32
+// rows of more than 512 experts 76 to 116.
 constexpr int kRouteBackThreads = 256;
 template <int V>
 constexpr int kRouteBackBlocks = V == 8 ? 4 : 2;        // resident on an SM
@@ -515,7 +517,7 @@ route_backward_kernel(const RowsIn logits, int64_t rows, int experts, int k, boo
 // Lanes of a row in the forward kernel.  Fewer lanes with more logits each make a warp's selections serve more rows (65536
 // rows in bf16: 128 experts by 8 lanes 22.5 us, by 16 26.7, by 4 28.8; 256 by 8 30.5, by 16 35.0, by 32
 // 37.1; 64 by 4 16.6, by 8 18.1), until a row's logits and sums fill the registers; from 257 experts on a whole
-// warp has its maximum in one instruction (16384 x 512: 21 us, by 16 lanes 25).
+// warp has its maximum in one instruction (16384 x 512: 21 us, by 16 lanes 25).  Measured with k = 8.
 constexpr int route_lanes(int experts) {
     return experts <= 8 ? 1 : experts <= 16 ? 2 : experts <= 64 ? 4 : experts <= 256 ? 8 : 32;
 }
@@ -579,7 +581,7 @@ static int route_most(int experts) {
     while (values * route_lanes(experts) < experts) values *= 2;
     return values == 8 ? kRouteMost<8> : values == 16 ? kRouteMost<16> : kRouteMost<32>;
 }
-// Threads of the forward kernel's blocks, and blocks: as many as have a row, at most one an SM (of 256 threads four).
+// Threads of the forward kernel's blocks, and blocks: as many as have a row, at most one an SM (of 256 threads two to four).
 static int route_threads(int device, int64_t rows, int experts) {
     const int most = route_most(experts);
     return rows * route_lanes(experts) / most < sm_count(device) ? kRouteFew : most;

@@ -18,7 +18,7 @@
 //
 // The values of the second block are written by its threads and read for a product that the first
 // block issues: its arrivals release, and the wait for them acquires, over the pair.  A warp of its own for each group's
-// arrivals keeps that release (some hundred cycles) out of the conversion: 8192 x 14336 x 4096 in 734 us, 751 with one such warp
+// arrivals keeps that release (most of a microsecond) out of the conversion: 8192 x 14336 x 4096 in 734 us, 751 with one such warp
 // for both groups, 770 with an arrival of every converting warp.
 //
 // A pair, because shared memory bounds a single block: for 256 x 256 x 64 its tensor
@@ -32,8 +32,8 @@
 // Rows behind a group's last are zeroed in both operands (a NaN of the next
 // group must not meet a zero).
 //
-// Bound by the tensor cores at the power limit and by the way from values to product: 8192 x 14336 x 4096 bf16 in 734 us,
-// 1311 TFLOP/s (cuBLAS on bf16 values 631 us).  A step of 64 rows takes 0.83 us for 1024 cycles of products.
+// Bound by the tensor cores at the power limit and by the way from values to product: 8192 x 14336 x 4096 bf16 in 730 us,
+// 1317 TFLOP/s (cuBLAS on bf16 values 629 us; 839 and 708 us in a loop of seconds, where both clock down).  A step of 64 rows takes 0.83 us for 1024 cycles of products.
 //
 // Work split: whole tiles go round the pairs, n-tiles outermost so that
 // pairs that run together share dy and codes in L2; the last wave and what
@@ -144,9 +144,9 @@ __device__ __forceinline__ int64_t wg_block_sum(int64_t v, int64_t* part) {
 }
 
 // Cutting evens the pairs' steps and costs the parts' way through memory and the second kernel, about as much
-// as this many steps: 4096 x 4096 x 4096, 128 tiles of 64 steps, takes 128 us cut over 74 pairs and 109 us as
-// two whole tiles on each of 64; 8192 x 14336 x 4096, 448 tiles of 128 steps, 690 us cut and 796 us in seven
-// rounds; 2048 x 768 x 768, 6 tiles of 32 steps, 30 us cut and 35 us whole.
+// as this many steps: 4096 x 4096 x 4096, 128 tiles of 64 steps, takes 145 us cut over 74 pairs and 123 us as
+// two whole tiles on each of 64; 8192 x 14336 x 4096, 448 tiles of 128 steps, 732 us cut and 769 us in seven
+// rounds; 2048 x 768 x 768, 6 tiles of 32 steps, 35 us cut and 38 us whole.
 constexpr int kWgCutSteps = 24;
 
 // This pair's segments.  Tiles [cut, tiles) are laid end to end as row steps; a pair
@@ -634,7 +634,7 @@ weight_grad_kernel(const __grid_constant__ CUtensorMap dy_map, const __grid_cons
 
 // Adds the parts of each cut tile, in the order of their rows.  Block (b, i): the tile whose first part
 // pair b left, rows [32 i, 32 i + 32).
-// 74 cut tiles of 512 x 256, two parts each, in 16 us from HBM.
+// 74 cut tiles of 512 x 256, two parts each, in 18 us from HBM.
 constexpr int kWgSlice = 32;
 
 template <int OT>

@@ -37,6 +37,8 @@
 extern "C" {
 #endif
 
+/* Raised with every change.  6 adds entry points to 5 and changes none of its structs,
+ * values or calls, so a caller built for 5 may accept 6. */
 #define AW4_ABI_VERSION 6
 #define AW4_BLOCK 128          /* elements per quantization block (4-bit default) */
 #define AW4_LUT_BINS 1024      /* maximum uniform bins over [-1, 1] for the rounding search */
