@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t warp_run(int run) {
 }
 
 // A lane reads 16 bytes of bf16 and writes 8 of codes; 32 blocks' exponents leave a warp together.  Bound by
-// HBM: 8192 x 14336 bf16 in 55 us, 6.5 TB/s (72 us with a capped grid whose warps had one run or two).
+// HBM: 8192 x 14336 bf16 in 55 to 60 us over several chips, 6.0 to 6.5 TB/s (72 us with a capped grid whose warps had one run or two).
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, uint8_t* __restrict__ codes,
@@ -65,7 +65,7 @@ act8_quantize_kernel(const RowsIn x, int64_t rows, int cols, uint32_t per_row, u
     store_scales(scales, unit0, units >> 2, b, lane);
 }
 
-// Bound by HBM: 8192 x 14336 bf16 in 51 us, 6.9 TB/s.
+// Bound by HBM: 8192 x 14336 bf16 in 52 us, 6.9 TB/s.
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows,
@@ -99,7 +99,7 @@ act8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restr
 // gated activation: h = g sigmoid(g) u
 // ---------------------------------------------------------------------------
 
-// float32 takes expf and a division: a few units in the last place, 0 once exp(-g) is above float32 (g < -88.8).  The
+// float32 takes expf and a division: a few units in the last place, 0 once exp(-g) is above float32 (g < -88.7).  The
 // 16-bit types take the hardware's exponential and reciprocal: off by (8 + 1.25 |g|) 2^-24 of the value, 0 from g < -87.4 on,
 // both far below their rounding.
 template <int DT>
@@ -114,11 +114,11 @@ __device__ __forceinline__ float sigmoid(float g) {
     }
 }
 
-// Chunks in flight: two forward (152 us at 8192 x 14336 bf16; 164 with one, 157 with four), one backward (149 us;
+// Chunks in flight: two forward (153 us at 8192 x 14336 bf16; 164 with one, 157 with four), one backward (145 us;
 // 167 with two, 205 with four).
 constexpr int kGluForward = 2, kGluBackward = 1;
 
-// Reads g and u, writes h and both checkpoints (EMIT: and that of h).  Bound by HBM: 8192 x 14336 bf16 in 152 us,
+// Reads g and u, writes h and both checkpoints (EMIT: and that of h).  Bound by HBM: 8192 x 14336 bf16 in 153 us,
 // 6.2 TB/s.
 template <int DT, bool WHOLE, bool EMIT>
 __global__ void __launch_bounds__(kA8Threads)
@@ -172,7 +172,7 @@ swiglu_forward_kernel(const RowsIn gate, const RowsIn up, int64_t rows, int cols
 }
 
 // dg = dh u (s + g s (1 - s)), du = dh g s, s = sigmoid(g), g and u from their checkpoints.  Bound by HBM:
-// 8192 x 14336 bf16 in 149 us, 6.4 TB/s.
+// 8192 x 14336 bf16 in 145 us, 6.5 TB/s.
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu_backward_kernel(const RowsIn dh, int64_t rows, int cols, uint32_t per_row,
@@ -324,7 +324,7 @@ struct NormWalk {
         t = threadIdx.x % NT;
     }
 };
-// Forward: 1024 threads of an SM at 64 registers (54 us at 16384 x 4096 bf16; 58 with 768, 64 with 512).
+// Forward: 1024 threads of an SM at 64 registers (55 us at 16384 x 4096 bf16; 58 with 768, 64 with 512).
 // Backward: 768 at 85 (61 us; 66 with 512, 103 with 1024, where its sums spill); 512 where what a thread has of
 // the next row is larger, in float32 and in the two chunks of a warp's row (2047 x 1531 float32: 14 us, 17 with 768).
 // Rows of more than 8192 values off 16 bytes, or 12288, need 1024 threads and spill all the same: 84 to 152 bytes a thread
@@ -333,7 +333,7 @@ constexpr int kNormForward = 1024, kNormBackwardMost = 768;
 template <int DT, int NT, int V>
 constexpr int kNormBackward = DT == AW4_F32 || (NT == 32 && V == 2) ? 512 : kNormBackwardMost;
 
-// Bound by HBM: 16384 x 4096 bf16 in 54 us, 6.2 TB/s.
+// Bound by HBM: 16384 x 4096 bf16 in 55 us, 6.2 TB/s.
 template <int DT, int NT, int V, bool WHOLE>
 __global__ void __launch_bounds__(NT <= 32 ? 32 * kNormWarps : NT, norm_blocks<NT>(kNormForward))
 rms_norm_forward_kernel(const RowsIn x, int64_t rows, int cols, float inv_cols, int per_row,
